@@ -281,6 +281,82 @@ WT_API int wt_logmel_pad_batch(const float *pcm, int n_chunks, int64_t n_samples
                                const float *mel_fb, int n_mels, int n_frames, float *mel_out, float *gmax,
                                int32_t *start_of_padding, void *stream);
 
+/* ---- A paged key-value cache and the attention of one new token over it ---------------------------------------------
+ * The reference has no cache of its own: it drives a backend that concatenates every layer's keys and values per token
+ * (T.py:783-793 only observes them).  These entries hold them in pages instead, so that sequences of different lengths
+ * step together and no token moves what is there already.
+ *
+ * A cache is n_pages pages of page_size slots for n_heads heads of head_dim values, keys and values apart.  Position p of
+ * sequence s lives in page table[s * table_stride + p / page_size], slot p % page_size; element d of head h of a key at
+ *     k[page * k_page_stride + h * k_head_stride + slot * k_slot_stride + d]                       (strides in elements)
+ * so (page, head, slot) may be laid out in any order.  Base addresses and strides are multiples of 16 bytes.
+ *   dtype F32 / F16 / BF16: the values as they are.
+ *   dtype E4M3: one byte a value and, per (page, head, slot), one byte E in k_exp / v_exp ([n_pages][n_heads][page_size],
+ *   contiguous): value = code * 2^(E - 127).  E is the least for which max |x| of the row <= 448 * 2^(E - 127) (at least
+ *   1); codes are x / 2^(E - 127) rounded to nearest even, so nothing but that rounding is lost.  Infinities and NaN are
+ *   stored as NaN and do not take part in the maximum.
+ * error (optional, device int32): a call that meets a sequence, position, length or page outside of its range never
+ * reads or writes there; it sets WT_KV_BAD_* bits here, and what it should have computed is NaN (what it should have
+ * written is not).  The caller clears the word. */
+#define WT_DTYPE_BF16 2
+#define WT_DTYPE_E4M3 3 /* the cache's pages only */
+
+#define WT_KV_BAD_POSITION 1 /* a position (append, gather) or a length (attend) outside of the table's row          */
+#define WT_KV_BAD_PAGE 2     /* a table entry in use outside of [0, n_pages)                                            */
+#define WT_KV_BAD_SEQUENCE 4 /* sequences[r] outside of [0, n_seqs)                                                     */
+
+typedef struct wt_kv_cache {
+    void *k;
+    void *v;
+    uint8_t *k_exp; /* E4M3 only, else NULL */
+    uint8_t *v_exp;
+    int64_t k_page_stride, k_head_stride, k_slot_stride;
+    int64_t v_page_stride, v_head_stride, v_slot_stride;
+    int32_t n_pages;
+    int32_t n_heads;
+    int32_t page_size; /* any from 1 */
+    int32_t head_dim;  /* 32, 64, 96, 128 or 256 */
+    int32_t dtype;
+    int32_t reserved;  /* 0 */
+    int32_t *error;
+} wt_kv_cache;
+
+/* Writes n_rows new rows: row r is position positions[r] of sequence sequences[r] (NULL: of sequence r; then
+ * n_rows <= n_seqs).  A row of negative position is a padded one: not written.  No two rows of a call may name the same
+ * place.  Slots that no row names keep what they hold.
+ *   k, v : device, element d of head h of row r at k[r * k_row_stride + h * k_head_stride + d]; multiples of 16 bytes;
+ *          dtype F32 / F16 / BF16: the cache's own, or any of them into an E4M3 cache
+ *   table: device int32, n_seqs rows of table_width entries, table_stride apart */
+WT_API int wt_kv_append(const wt_kv_cache *cache, const void *k, const void *v, int dtype, int64_t k_row_stride, int64_t k_head_stride,
+                        int64_t v_row_stride, int64_t v_head_stride, int n_rows, const int32_t *table, int64_t table_stride,
+                        int n_seqs, int table_width, const int32_t *sequences, const int32_t *positions, void *stream);
+
+/* Reads rows back: k[r][h][:] (contiguous [n_rows][n_heads][head_dim]) = the key at positions[r] of sequence sequences[r],
+ * in dtype: the cache's own, or F32 / F16 / BF16 (rounded to nearest even once) from an E4M3 cache.  A row of negative position
+ * reads as zeros, one outside of its range as NaN. */
+WT_API int wt_kv_gather(const wt_kv_cache *cache, void *k, void *v, int dtype, int n_rows, const int32_t *table, int64_t table_stride,
+                        int n_seqs, int table_width, const int32_t *sequences, const int32_t *positions, void *stream);
+
+/* One new token of every sequence over its cached positions 0 ... lengths[s] - 1 (write the token's own key and value
+ * first for it to see itself).  Query head h reads key head h / (n_q_heads / n_heads):
+ *     w_t = scale * q . k_t,   out = sum_t exp(w_t - max w) v_t / sum_t exp(w_t - max w),   lse = log sum_t exp(w_t)
+ * Products are summed, and maximum, sum and result held, in 32 bits; out is rounded once.  lengths[s] = 0: out = 0, lse =
+ * -inf.  What pages hold behind the last position takes no part, NaN and infinities included; an infinity among the values
+ * that do take part leaves its element infinite or NaN.
+ *   q, out : device, dtype F32 / F16 / BF16 (the cache's own; any of them over an E4M3 cache), head_dim values in a row;
+ *            out may be q.  Rows beyond n_seqs are not touched
+ *   lse    : optional device fp32 [n_seqs][n_q_heads]
+ *   workspace : wt_kv_attend_workspace() bytes of device memory, 16-byte aligned, zeroed once before its first use; every
+ *            call leaves it ready for the next one.  Two calls that may run at the same time (on two streams, or in two
+ *            graphs) need one each.  NULL: the library's arena of this stream; refused while the stream is capturing */
+WT_API int wt_kv_attend(const wt_kv_cache *cache, const void *q, int dtype, int64_t q_row_stride, int64_t q_head_stride, int n_seqs,
+                        int n_q_heads, float scale, const int32_t *table, int64_t table_stride, int table_width,
+                        const int32_t *lengths, void *out, int64_t out_row_stride, int64_t out_head_stride, float *lse,
+                        void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Bytes of workspace that wt_kv_attend needs on the current device for this cache and these counts (< 0: error). */
+WT_API int64_t wt_kv_attend_workspace(const wt_kv_cache *cache, int n_seqs, int n_q_heads, int table_width);
+
 #ifdef __cplusplus
 }
 #endif

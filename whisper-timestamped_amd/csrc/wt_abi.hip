@@ -98,6 +98,13 @@ int capture_rows(const void *, int, int, int, int, const int32_t *, const int32_
                  hipStream_t);
 int qk_rows(const void *, const void *, int, int, int, int, int, float, const int32_t *, const int32_t *, int, void *, int,
             int64_t, int64_t, hipStream_t);
+int kv_append(const wt_kv_cache *, const void *, const void *, int, int64_t, int64_t, int64_t, int64_t, int, const int32_t *, int64_t,
+              int, int, const int32_t *, const int32_t *, hipStream_t);
+int kv_gather(const wt_kv_cache *, void *, void *, int, int, const int32_t *, int64_t, int, int, const int32_t *, const int32_t *,
+              hipStream_t);
+int kv_attend(const wt_kv_cache *, const void *, int, int64_t, int64_t, int, int, float, const int32_t *, int64_t, int, const int32_t *,
+              void *, int64_t, int64_t, float *, void *, int64_t, hipStream_t);
+int64_t kv_attend_workspace(const wt_kv_cache *, int, int, int);
 
 }  // namespace wt
 
@@ -279,6 +286,31 @@ int wt_logmel_pad_batch(const float *pcm, int n_chunks, int64_t n_samples, const
     }
     return wt::logmel_batch(pcm, n_chunks, n_samples, n_valid_samples, mel_fb, n_mels, n_frames, mel_out, gmax, start_of_padding,
                             (hipStream_t)stream);
+}
+
+int wt_kv_append(const wt_kv_cache *cache, const void *k, const void *v, int dtype, int64_t k_row_stride, int64_t k_head_stride,
+                 int64_t v_row_stride, int64_t v_head_stride, int n_rows, const int32_t *table, int64_t table_stride, int n_seqs,
+                 int table_width, const int32_t *sequences, const int32_t *positions, void *stream) {
+    return wt::kv_append(cache, k, v, dtype, k_row_stride, k_head_stride, v_row_stride, v_head_stride, n_rows, table, table_stride,
+                         n_seqs, table_width, sequences, positions, (hipStream_t)stream);
+}
+
+int wt_kv_gather(const wt_kv_cache *cache, void *k, void *v, int dtype, int n_rows, const int32_t *table, int64_t table_stride,
+                 int n_seqs, int table_width, const int32_t *sequences, const int32_t *positions, void *stream) {
+    return wt::kv_gather(cache, k, v, dtype, n_rows, table, table_stride, n_seqs, table_width, sequences, positions,
+                         (hipStream_t)stream);
+}
+
+int wt_kv_attend(const wt_kv_cache *cache, const void *q, int dtype, int64_t q_row_stride, int64_t q_head_stride, int n_seqs,
+                 int n_q_heads, float scale, const int32_t *table, int64_t table_stride, int table_width, const int32_t *lengths,
+                 void *out, int64_t out_row_stride, int64_t out_head_stride, float *lse, void *workspace, int64_t workspace_bytes,
+                 void *stream) {
+    return wt::kv_attend(cache, q, dtype, q_row_stride, q_head_stride, n_seqs, n_q_heads, scale, table, table_stride, table_width,
+                         lengths, out, out_row_stride, out_head_stride, lse, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int64_t wt_kv_attend_workspace(const wt_kv_cache *cache, int n_seqs, int n_q_heads, int table_width) {
+    return wt::kv_attend_workspace(cache, n_seqs, n_q_heads, table_width);
 }
 
 }  // extern "C"

@@ -16,7 +16,7 @@ _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 # (WT_LIBWTALIGN: another build of the same library, for A/B measurements of kernel variants -- tools/ab_cost.py)
 LIB_PATH = os.environ.get("WT_LIBWTALIGN") or os.path.join(_PKG_ROOT, "libwtalign.so")
 
-WT_DTYPE_F32, WT_DTYPE_F16 = 0, 1
+WT_DTYPE_F32, WT_DTYPE_F16, WT_DTYPE_BF16, WT_DTYPE_E4M3 = 0, 1, 2, 3
 WT_MAX_TOKENS, WT_MAX_FRAMES = 256, 1792
 N_AUDIO_CTX = 1500
 
@@ -31,10 +31,21 @@ assert SEG_DTYPE.itemsize == 64
 EXPORTS = ["wt_version", "wt_last_error", "wt_shutdown", "wt_cost_batch", "wt_dtw_batch", "wt_align_batch",
            "wt_find_start_padding_batch", "wt_logprob_gather_batch", "wt_logmel_batch", "wt_capture_rows", "wt_qk_rows",
            "wt_disfluency_batch", "wt_qk_rows_batch", "wt_logprob_gather_rows", "wt_dtw_batch_pattern", "wt_align_batch_v3",
-           "wt_release_stream", "wt_qk_rows_streams", "wt_logmel_pad_batch", "wt_logprob_digest_streams"]
+           "wt_release_stream", "wt_qk_rows_streams", "wt_logmel_pad_batch", "wt_logprob_digest_streams",
+           "wt_kv_append", "wt_kv_gather", "wt_kv_attend", "wt_kv_attend_workspace"]
 WT_STEP_SYMMETRIC1, WT_STEP_NO_EMPTY_SUBWORDS = 0, 1
 ABI_VERSION = 5
+WT_KV_BAD_POSITION, WT_KV_BAD_PAGE, WT_KV_BAD_SEQUENCE = 1, 2, 4
 WT_ALIGN_KEEP_COST, WT_ALIGN_NO_FUSED_SMALL_UNITS, WT_ALIGN_ROWS_PER_CLASS = 1, 2, 4
+
+
+class KvCache(ctypes.Structure):
+    """mirrors `struct wt_kv_cache`"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p),
+                ("k_page_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64), ("k_slot_stride", ctypes.c_int64),
+                ("v_page_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("v_slot_stride", ctypes.c_int64),
+                ("n_pages", ctypes.c_int32), ("n_heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("error", ctypes.c_void_p)]
 
 
 class WtError(RuntimeError):
@@ -76,11 +87,19 @@ def load():
     L.wt_qk_rows_streams.argtypes = [vp, vp, i32, i32, i32, i32, i64, i64, i32, i32, i32, f32, vp, vp, vp, i32, vp, vp, i32, i64,
                                      i64, i64, vp]
     L.wt_logprob_digest_streams.argtypes = [vp, i64, i32, i32, vp, i32, i64, vp, i64, i64, vp, i32, i32, vp, vp, vp]
+    missing = [n for n in EXPORTS if not hasattr(L, n)]      # (entries may be added within an ABI version)
+    if missing:
+        raise ImportError(f"{LIB_PATH} lacks {', '.join(missing)}: rebuild it (`make -C {_PKG_ROOT}/csrc`)")
+    L.wt_kv_append.argtypes = [vp, vp, vp, i32, i64, i64, i64, i64, i32, vp, i64, i32, i32, vp, vp, vp]
+    L.wt_kv_gather.argtypes = [vp, vp, vp, i32, i32, vp, i64, i32, i32, vp, vp, vp]
+    L.wt_kv_attend.argtypes = [vp, vp, i32, i64, i64, i32, i32, f32, vp, i64, i32, vp, vp, i64, i64, vp, vp, i64, vp]
+    L.wt_kv_attend_workspace.argtypes = [vp, i32, i32, i32]
     if L.wt_version() != ABI_VERSION:
         raise ImportError(f"{LIB_PATH} exports ABI version {L.wt_version()}, this package needs {ABI_VERSION}: rebuild it "
                           f"(`make -C {_PKG_ROOT}/csrc`)")
     for n in EXPORTS[3:]:
         getattr(L, n).restype = i32
+    L.wt_kv_attend_workspace.restype = i64
     _lib = L
     return L
 
