@@ -305,6 +305,8 @@ WT_API int wt_logmel_pad_batch(const float *pcm, int n_chunks, int64_t n_samples
 #define WT_KV_BAD_PAGE 2     /* a table entry in use outside of [0, n_pages)                                            */
 #define WT_KV_BAD_SEQUENCE 4 /* sequences[r] outside of [0, n_seqs)                                                     */
 
+#define WT_KV_WORKSPACE_ZEROED 16384 /* leading bytes of wt_kv_attend's workspace that have to be zero                   */
+
 typedef struct wt_kv_cache {
     void *k;
     void *v;
@@ -346,8 +348,8 @@ WT_API int wt_kv_gather(const wt_kv_cache *cache, void *k, void *v, int dtype, i
  *   q, out : device, dtype F32 / F16 / BF16 (the cache's own; any of them over an E4M3 cache), head_dim values in a row;
  *            out may be q.  Rows beyond n_seqs are not touched
  *   lse    : optional device fp32 [n_seqs][n_q_heads]
- *   workspace : wt_kv_attend_workspace() bytes of device memory, 16-byte aligned, zeroed once before its first use; every
- *            call leaves it ready for the next one.  Two calls that may run at the same time (on two streams, or in two
+ *   workspace : wt_kv_attend_workspace() bytes of device memory, 16-byte aligned, its first WT_KV_WORKSPACE_ZEROED bytes zeroed
+ *            once before its first use; every call leaves it ready for the next one.  Two calls that may run at the same time (on two streams, or in two
  *            graphs) need one each.  NULL: the library's arena of this stream; refused while the stream is capturing */
 WT_API int wt_kv_attend(const wt_kv_cache *cache, const void *q, int dtype, int64_t q_row_stride, int64_t q_head_stride, int n_seqs,
                         int n_q_heads, float scale, const int32_t *table, int64_t table_stride, int table_width,

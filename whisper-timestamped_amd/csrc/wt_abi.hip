@@ -73,6 +73,16 @@ int scratch_tagged(hipStream_t st, size_t bytes, void **out, const void *tag_ptr
     a->tag_val = tag_val;
     return WT_OK;
 }
+// workspace of wt_kv_attend; `fresh`: new memory, whose counters the caller has to clear on `st`
+int scratch_kv(hipStream_t st, size_t bytes, void **out, bool *fresh) {
+    Arena *a = nullptr;
+    const int rc = scratch_ex(3, st, bytes, out, &a);
+    if (rc) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    *fresh = a->tag_val != 1;
+    a->tag_val = 1;
+    return WT_OK;
+}
 void scratch_forget_tags() {
     std::lock_guard<std::mutex> lk(g_mu);
     for (auto &kv : g_arena) kv.second.tag_ptr = nullptr;

@@ -1,99 +1,8 @@
 // A paged key-value cache: writing it (plain, or in 8 bits with one power of two per row), reading it back, and the
 // attention of one new token per sequence over it.  Layout and formulas: include/wtalign.h, wt_kv_*.
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
-
-#include "wt_common.h"
+#include "wt_kv.h"
 
 namespace wt {
-
-// position -> (page index, slot) for any page size: q = (p * m) >> s with m = ceil(2^s / d), s = 31 + ceil(log2 d), is exact
-// for 0 <= p < 2^31 and m < 2^32
-struct PageDiv {
-    uint32_t d, m, s;
-};
-static PageDiv page_div(int d) {
-    PageDiv r = {(uint32_t)d, 0, 31};
-    while ((1ull << (r.s - 31)) < (uint64_t)d) ++r.s;
-    r.m = (uint32_t)(((1ull << r.s) + d - 1) / d);   // d = 1: 2^31
-    return r;
-}
-__device__ __forceinline__ uint32_t page_of(PageDiv v, uint32_t p) { return (uint32_t)(((uint64_t)p * v.m) >> v.s); }
-
-struct KvRows {   // one of the two tensors of a cache
-    void *p;
-    uint8_t *e;
-    int64_t page, head, slot;   // strides in elements
-};
-struct KvDims {
-    int n_pages, n_heads, page_size, head_dim;
-    PageDiv div;
-    int32_t *error;
-};
-struct KvTable {
-    const int32_t *t;
-    int64_t stride;
-    int n_seqs, width;
-};
-
-__device__ __forceinline__ void kv_report(int32_t *error, int bits) {
-    if (error) atomicOr(error, bits);
-}
-
-// Page and slot of position `pos` of sequence `seq`; false (and the error word) where one of them is out of range.
-__device__ __forceinline__ bool kv_place(const KvDims &c, const KvTable &t, int seq, int pos, int *page, int *slot) {
-    if ((uint32_t)seq >= (uint32_t)t.n_seqs) {
-        kv_report(c.error, WT_KV_BAD_SEQUENCE);
-        return false;
-    }
-    const uint32_t pi = page_of(c.div, (uint32_t)pos);
-    if (pi >= (uint32_t)t.width) {
-        kv_report(c.error, WT_KV_BAD_POSITION);
-        return false;
-    }
-    *page = t.t[(int64_t)seq * t.stride + pi];
-    *slot = pos - (int)(pi * c.div.d);
-    if ((uint32_t)*page >= (uint32_t)c.n_pages) {
-        kv_report(c.error, WT_KV_BAD_PAGE);
-        return false;
-    }
-    return true;
-}
-
-// ---- types ----------------------------------------------------------------------------------------------------------
-typedef float f4 __attribute__((ext_vector_type(4)));
-struct fp8_t {
-    uint8_t b;
-};
-struct bf16_t {
-    uint16_t b;
-};
-struct f16_t {
-    uint16_t b;
-};
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(f16_t v) { return __half2float(__ushort_as_half(v.b)); }
-__device__ __forceinline__ float to_f(bf16_t v) { return __uint_as_float((uint32_t)v.b << 16); }
-__device__ __forceinline__ float to_f(fp8_t v) { return __builtin_amdgcn_cvt_f32_fp8((int)v.b, 0); }
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ f16_t from_f<f16_t>(float v) { return {__half_as_ushort(__float2half(v))}; }
-template <>
-__device__ __forceinline__ bf16_t from_f<bf16_t>(float v) {   // round to nearest even, NaN stays NaN
-    const uint32_t u = __float_as_uint(v);
-    return {(uint16_t)((u & 0x7fffffffu) > 0x7f800000u ? (u >> 16) | 0x40u : (u + 0x7fffu + ((u >> 16) & 1u)) >> 16)};
-}
-// the power of two that a stored exponent byte stands for (0, which no row of a written cache has, stands for 0)
-__device__ __forceinline__ float exp_of(uint32_t e) { return __uint_as_float(e << 23); }
-
-template <typename T, int N>
-struct alignas((sizeof(T) * N & -(sizeof(T) * N)) > 16 ? 16 : sizeof(T) * N & -(sizeof(T) * N)) Pack {   // N elements that travel together
-    T v[N];
-};
-static_assert(sizeof(Pack<float, 6>) == 24 && sizeof(Pack<uint16_t, 6>) == 12 && sizeof(Pack<uint16_t, 8>) == 16, "no padding");
 
 // ---- writing rows ---------------------------------------------------------------------------------------------------
 // A row (one head of one token) is HD values; LPR lanes take EPL = HD / LPR of them each, so that a lane moves 16 bytes of
@@ -212,78 +121,6 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvRows k, KvRows v, KvDi
     kv_load_row<DT, CT, HD>(v, vd + to, page * v.page + h * v.head + slot * v.slot, eoff, ok, fill, lane);
 }
 
-// ---- attention of one new token ---------------------------------------------------------------------------------------
-// One workgroup per (sequence, query head); a wave takes every fourth run of 64 positions, a lane one key of the run: its
-// score, the run's maximum and sum by wave reductions, then all lanes over the run's values, HD / 64 columns each.
-constexpr int KV_NEG_WAVES = 4;
-template <typename T, typename CT>
-__global__ __launch_bounds__(256) void kv_attend_kernel(KvRows k, KvRows v, KvDims c, KvTable t, const T *__restrict__ q, int64_t q_row,
-                                                        int64_t q_head, int n_q_heads, float scale,
-                                                        const int32_t *__restrict__ lengths, T *__restrict__ out, int64_t o_row,
-                                                        int64_t o_head, float *__restrict__ lse) {
-    __shared__ float qs[256], part[KV_NEG_WAVES][256], pm[KV_NEG_WAVES], pl[KV_NEG_WAVES];
-    const int s = blockIdx.x / n_q_heads, hq = blockIdx.x % n_q_heads, h = hq / (n_q_heads / c.n_heads);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hd = c.head_dim;
-    if ((int)threadIdx.x < hd) qs[threadIdx.x] = to_f(q[s * q_row + hq * q_head + threadIdx.x]);
-    int len = lengths[s];
-    bool bad = false;
-    if (len < 0 || len > (int64_t)t.width * c.page_size) {
-        if (threadIdx.x == 0) kv_report(c.error, WT_KV_BAD_POSITION);
-        bad = true;
-        len = 0;
-    }
-    __syncthreads();
-    const float LOWEST = -3.402823466e38f;
-    float m = LOWEST, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = wave * 64; p0 < len; p0 += KV_NEG_WAVES * 64) {
-        const int pos = p0 + lane;
-        const bool in = pos < len;
-        int page = 0, slot = 0;
-        const bool ok = in && kv_place(c, t, s, pos, &page, &slot);
-        bad |= in && !ok;
-        float x = -__builtin_inff(), ve = 0.f;
-        if (ok) {
-            const CT *row = static_cast<const CT *>(k.p) + page * k.page + h * k.head + slot * k.slot;
-            float a = 0.f;
-            for (int d = 0; d < hd; ++d) a = fmaf(qs[d], to_f(row[d]), a);
-            if constexpr (sizeof(CT) == 1) {
-                const int64_t eo = ((int64_t)page * c.n_heads + h) * c.page_size + slot;
-                a *= exp_of(k.e[eo]);
-                ve = exp_of(v.e[eo]);
-            } else
-                ve = 1.f;
-            x = a * scale;
-        }
-        const float mn = fmaxf(m, wave_max(x)), f = expf(m - mn), p = ok ? expf(x - mn) : 0.f;
-        l = l * f + wave_sum(p);
-        m = mn;
-        for (int i = 0; i < 4; ++i) o[i] *= f;
-        const int n = min(64, len - p0);
-        for (int j = 0; j < n; ++j) {
-            if (!__shfl((int)ok, j, 64)) continue;
-            const float pj = __shfl(p, j, 64) * __shfl(ve, j, 64);
-            const CT *row = static_cast<const CT *>(v.p) + __shfl(page, j, 64) * v.page + h * v.head + __shfl(slot, j, 64) * v.slot;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (lane + i * 64 < hd) o[i] = fmaf(pj, to_f(row[lane + i * 64]), o[i]);
-        }
-    }
-    if (__any(bad)) l = __builtin_nanf("");
-    for (int i = 0; i < 4; ++i)
-        if (lane + i * 64 < hd) part[wave][lane + i * 64] = o[i];
-    if (lane == 0) pm[wave] = m, pl[wave] = l;
-    __syncthreads();
-    float mm = LOWEST, ll = 0.f;
-    for (int w = 0; w < KV_NEG_WAVES; ++w) mm = fmaxf(mm, pm[w]);
-    for (int w = 0; w < KV_NEG_WAVES; ++w) ll += pl[w] * expf(pm[w] - mm);
-    if ((int)threadIdx.x < hd) {
-        float a = 0.f;
-        for (int w = 0; w < KV_NEG_WAVES; ++w) a += part[w][threadIdx.x] * expf(pm[w] - mm);
-        out[s * o_row + hq * o_head + threadIdx.x] = from_f<T>(len == 0 && ll == 0.f ? 0.f : a / ll);
-    }
-    if (lse && threadIdx.x == 0) lse[(int64_t)s * n_q_heads + hq] = mm + logf(ll);
-}
-
 // ---- host -----------------------------------------------------------------------------------------------------------
 static int kv_check(const char *what, const wt_kv_cache *c, int dtype, const int32_t *table, int64_t table_stride, int n_seqs,
                     int table_width) {
@@ -314,6 +151,10 @@ static int kv_check(const char *what, const wt_kv_cache *c, int dtype, const int
         }
     if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) {
         set_error("%s: the cache's pages are not 16-byte aligned", what);
+        return WT_E_BADARG;
+    }
+    if (((uintptr_t)c->k_exp | (uintptr_t)c->v_exp) & 15) {
+        set_error("%s: the exponents are not 16-byte aligned", what);
         return WT_E_BADARG;
     }
     if (!table || n_seqs < 0 || table_width <= 0 || (n_seqs > 1 && table_stride < table_width) ||
@@ -405,27 +246,111 @@ int kv_gather(const wt_kv_cache *c, void *k, void *v, int dtype, int n_rows, con
     return WT_OK;
 }
 
-int64_t kv_attend_workspace(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_width) { return 0; }
+// ---- attention of one new token: schedule ------------------------------------------------------------------------------
+int scratch_kv(hipStream_t st, size_t bytes, void **out, bool *fresh);
+int kv_attend_f32(const KvAttend &, unsigned, hipStream_t);
+int kv_attend_f16(const KvAttend &, unsigned, hipStream_t);
+int kv_attend_bf16(const KvAttend &, unsigned, hipStream_t);
+int kv_attend_e4m3_f32(const KvAttend &, unsigned, hipStream_t);
+int kv_attend_e4m3_f16(const KvAttend &, unsigned, hipStream_t);
+int kv_attend_e4m3_bf16(const KvAttend &, unsigned, hipStream_t);
+
+__global__ void kv_zero_kernel(int32_t *p) { p[blockIdx.x * 256 + threadIdx.x] = 0; }
+
+struct KvPlan {
+    int direct, n_wg, min_share;
+    unsigned grid;
+    int64_t bytes;
+};
+
+static int kv_plan(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_width, KvPlan *p) {
+    static int cus[16] = {0};   // per device; two threads that fill it write the same
+    int dev = 0;
+    WT_HIP(hipGetDevice(&dev));
+    int n = dev < 16 ? cus[dev] : 0;
+    if (n == 0) {
+        WT_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
+        if (dev < 16) cus[dev] = n;
+    }
+    const int unit = c->dtype == WT_DTYPE_F32 ? 64 : 128, group = n_q_heads / c->n_heads;
+    const int64_t pairs = (int64_t)n_seqs * c->n_heads * ((group + 15) / 16);
+    p->n_wg = n * 2 < WT_KV_WORKSPACE_ZEROED / 4 ? n * 2 : WT_KV_WORKSPACE_ZEROED / 4;
+    p->min_share = 4;
+    p->direct = (int64_t)table_width * c->page_size <= (int64_t)p->min_share * unit;
+    p->grid = p->direct ? (unsigned)pairs : (unsigned)p->n_wg;
+    p->bytes = p->direct ? 0 : WT_KV_WORKSPACE_ZEROED + (int64_t)p->n_wg * 2 * (32 + 16 * c->head_dim) * 4;
+    return WT_OK;
+}
+
+static int kv_check_heads(const wt_kv_cache *c, int n_seqs, int n_q_heads) {
+    if (n_q_heads <= 0 || n_q_heads % c->n_heads != 0 || (int64_t)n_seqs * n_q_heads > 0x7fffffffll) {
+        set_error("wt_kv_attend: %d query heads over %d key heads, %d sequences", n_q_heads, c->n_heads, n_seqs);
+        return WT_E_BADARG;
+    }
+    return WT_OK;
+}
+
+int64_t kv_attend_workspace(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_width) {
+    static const int32_t none = 0;
+    int rc = kv_check("wt_kv_attend_workspace", c, c && c->dtype != WT_DTYPE_E4M3 ? c->dtype : 0, &none, table_width, n_seqs, table_width);
+    if (!rc) rc = kv_check_heads(c, n_seqs, n_q_heads);
+    KvPlan p;
+    if (!rc) rc = kv_plan(c, n_seqs, n_q_heads, table_width, &p);
+    return rc ? rc : p.bytes;
+}
 
 int kv_attend(const wt_kv_cache *c, const void *q, int dtype, int64_t q_row, int64_t q_head, int n_seqs, int n_q_heads, float scale,
               const int32_t *table, int64_t table_stride, int table_width, const int32_t *lengths, void *out, int64_t o_row,
               int64_t o_head, float *lse, void *workspace, int64_t workspace_bytes, hipStream_t st) {
-    const int rc = kv_check("wt_kv_attend", c, dtype, table, table_stride, n_seqs, table_width);
+    int rc = kv_check("wt_kv_attend", c, dtype, table, table_stride, n_seqs, table_width);
     if (rc) return rc;
-    if (!q || !out || !lengths || n_q_heads <= 0 || n_q_heads % c->n_heads != 0 || (int64_t)n_seqs * n_q_heads > 0x7fffffffll) {
-        set_error("wt_kv_attend: null pointer, or %d query heads over %d key heads", n_q_heads, c->n_heads);
+    if (!q || !out || !lengths) {
+        set_error("wt_kv_attend: null pointer");
         return WT_E_BADARG;
     }
+    if ((rc = kv_check_heads(c, n_seqs, n_q_heads))) return rc;
+    const int64_t item = dtype == WT_DTYPE_F32 ? 4 : 2, held = c->dtype == WT_DTYPE_E4M3 ? 1 : item;
+    if (((uintptr_t)q | (uintptr_t)out) & (item - 1)) {
+        set_error("wt_kv_attend: q or out is not aligned to its elements");
+        return WT_E_BADARG;
+    }
+    if ((c->k_slot_stride > c->v_slot_stride ? c->k_slot_stride : c->v_slot_stride) * held * 32 > 0x7fffffffll) {
+        set_error("wt_kv_attend: slots of a page are too far apart");
+        return WT_E_UNSUPPORTED;
+    }
     if (n_seqs == 0) return WT_OK;
-#define WT_KV_GO(T, CT)                                                                                                              \
-    hipLaunchKernelGGL((kv_attend_kernel<T, CT>), dim3((unsigned)(n_seqs * n_q_heads)), dim3(256), 0, st, kv_k(c), kv_v(c), kv_dims(c), \
-                       (KvTable{table, table_stride, n_seqs, table_width}), (const T *)q, q_row, q_head, n_q_heads, scale, lengths, (T *)out, \
-                       o_row, o_head, lse)
-#define WT_KV_ONE(F, A, B) { F(A, B); }
-    WT_KV_TYPES(WT_KV_ONE, WT_KV_GO)
-#undef WT_KV_GO
-    WT_HIP(hipGetLastError());
-    return WT_OK;
+    KvPlan p;
+    if ((rc = kv_plan(c, n_seqs, n_q_heads, table_width, &p))) return rc;
+    if (p.bytes > 0) {
+        if (workspace) {
+            if (workspace_bytes < p.bytes || ((uintptr_t)workspace & 15)) {
+                set_error("wt_kv_attend: workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)p.bytes);
+                return WT_E_BADARG;
+            }
+        } else {
+            hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+            WT_HIP(hipStreamIsCapturing(st, &cap));
+            if (cap != hipStreamCaptureStatusNone) {
+                set_error("wt_kv_attend: a captured call needs a workspace of its own (%lld bytes)", (long long)p.bytes);
+                return WT_E_BADARG;
+            }
+            bool fresh = false;
+            if ((rc = scratch_kv(st, (size_t)p.bytes, &workspace, &fresh))) return rc;
+            if (fresh) hipLaunchKernelGGL(kv_zero_kernel, dim3(WT_KV_WORKSPACE_ZEROED / 1024), dim3(256), 0, st, (int32_t *)workspace);
+        }
+    }
+    KvAttend a;
+    a.k = kv_k(c), a.v = kv_v(c), a.c = kv_dims(c), a.t = KvTable{table, table_stride, n_seqs, table_width};
+    a.q = q, a.q_row = q_row, a.q_head = q_head;
+    a.n_q_heads = n_q_heads, a.group = n_q_heads / c->n_heads, a.q_tiles = (a.group + 15) / 16;
+    a.scale = scale, a.lengths = lengths, a.out = out, a.o_row = o_row, a.o_head = o_head, a.lse = lse;
+    a.q_aligned = (((uintptr_t)q | (uint64_t)(q_row * item) | (uint64_t)(q_head * item)) & 15) == 0;
+    a.direct = p.direct, a.n_wg = p.n_wg, a.min_share = p.min_share;
+    a.counters = (int32_t *)workspace;
+    a.partials = workspace ? (float *)((char *)workspace + WT_KV_WORKSPACE_ZEROED) : nullptr;
+    if (c->dtype == WT_DTYPE_E4M3)
+        return dtype == WT_DTYPE_F32 ? kv_attend_e4m3_f32(a, p.grid, st) : dtype == WT_DTYPE_F16 ? kv_attend_e4m3_f16(a, p.grid, st) : kv_attend_e4m3_bf16(a, p.grid, st);
+    return dtype == WT_DTYPE_F32 ? kv_attend_f32(a, p.grid, st) : dtype == WT_DTYPE_F16 ? kv_attend_f16(a, p.grid, st) : kv_attend_bf16(a, p.grid, st);
 }
 
 }  // namespace wt

@@ -1,0 +1,596 @@
+// The attention of one new token over the paged cache: the kernel, instantiated per type by wt_kv_attend_*.hip.
+#pragma once
+#include "wt_kv.h"
+
+namespace wt {
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float fl2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr float KV_LOWEST = -3.402823466e38f;   // the running maximum's start: finite, so x - m is never inf - inf
+constexpr float KV_LOG2E = 1.44269504088896340736f;
+
+// CT: what the pages hold; T: queries and results.
+// Matrix instructions take 16-bit operands as they are; 8-bit codes become bf16 (exactly), and then the queries are split
+// into bf16 parts whose sum they are: bf16 1, f16 2, f32 3.  f32 pages use the f32 instruction.
+template <typename CT, typename T>
+struct KvKind {
+    static constexpr bool F32 = sizeof(CT) == 4, E4M3 = sizeof(CT) == 1;
+    static constexpr bool F16 = !F32 && !E4M3 && __is_same(CT, f16_t);
+    static constexpr int KB = F32 ? 16 : 32;                // keys a wave takes at a time
+    static constexpr int NT = KB / 16;                      // ... in tiles of 16
+    static constexpr int GK = KB / 4;                       // keys a lane group holds the weights and values of
+    static constexpr int QP = !E4M3 ? 1 : __is_same(T, bf16_t) ? 1 : __is_same(T, f16_t) ? 2 : 3;
+    // f16 weights are kept away from f16's subnormal numbers: the reference of the exponentials sits BIAS below the maximum
+    // seen, which may be outgrown by SLACK before it moves; exp(BIAS + SLACK) < 65504
+    static constexpr float BIAS = F16 ? 5.5f : 0.f, SLACK = F16 ? 5.5f : 8.f;
+};
+
+// d index of the first of the 8 (f32: 4) elements that lane group g takes of contraction step s; K and Q use the same one.
+// 8-bit pages: two steps of a full 64 share one 16-byte load.
+template <typename CT, int HD>
+__device__ __forceinline__ constexpr int kv_d(int s, int g) {
+    if (sizeof(CT) == 4) return s * 16 + g * 4;
+    if (sizeof(CT) == 1 && (s / 2 + 1) * 64 <= HD) return s / 2 * 64 + g * 16 + (s & 1) * 8;
+    return s * 32 + g * 8;
+}
+
+template <typename CT, typename T, int HD>
+struct KvFrag {
+    using K = KvKind<CT, T>;
+    static constexpr int STEPS = HD / (K::F32 ? 16 : 32), EV = HD / 16;
+    static constexpr int KD = K::E4M3 ? 2 : 4;                                       // dwords a step and tile
+    static constexpr int VD = (EV * (int)sizeof(CT) + 3) / 4;                        // dwords of a key's values
+    uint32_t k[K::NT][STEPS][KD];
+    uint32_t v[K::GK][VD];
+    uint2 ke, ve;                                                                    // 8-bit pages: exponents of the lane group's 8 keys
+};
+
+template <int N>   // N bytes from a place aligned to as many of them as a power of two allows (16 at most)
+__device__ __forceinline__ void kv_fetch(uint32_t *dst, const char *src) {
+    if constexpr (N == 2) dst[0] = *reinterpret_cast<const uint16_t *>(src);
+    else if constexpr (N == 6) {
+        const uint16_t *s = reinterpret_cast<const uint16_t *>(src);
+        dst[0] = s[0] | (uint32_t)s[1] << 16, dst[1] = s[2];
+    } else if constexpr (N <= 16 || N == 24) {
+        constexpr int D = N / 4;
+        using P = Pack<uint32_t, D>;
+        const P p = *reinterpret_cast<const P *>(src);
+#pragma unroll
+        for (int i = 0; i < D; ++i) dst[i] = p.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 16; ++i) kv_fetch<16>(dst + 4 * i, src + 16 * i);
+    }
+}
+
+// Where a block's rows are, for this lane: byte offsets from the tensors' starts.
+//   PG 32: a page size that 32 divides: the block is in one page, the offsets the wave's
+//   PG  8: one that 8 divides (f32: 4): each group of keys is in one page
+//   PG  1: any other: each key by itself
+template <int PG, int NT, int GK>
+struct KvSpot {
+    int64_t k[PG == 1 ? NT : 1], v[PG == 1 ? GK : 1];
+    int64_t e[PG == 1 ? GK : 1];
+};
+
+template <typename CT, typename T, int HD, int PG, int NW>
+struct KvWave {
+    using K = KvKind<CT, T>;
+    using Frag = KvFrag<CT, T, HD>;
+    using Spot = KvSpot<PG, K::NT, K::GK>;
+    static constexpr int STEPS = Frag::STEPS, EV = Frag::EV, ITEM = sizeof(CT);
+
+    const KvAttend &a;
+    const int lane, g, n;
+    const int32_t *row;   // the sequence's row of the table
+    int len, h;
+    bool bad = false;
+    uint32_t koff, voff;  // PG 32: this lane's byte offsets inside a page
+    // queries
+    u4 q[K::F32 ? 1 : K::QP][K::F32 ? 1 : STEPS];
+    f4 qf[K::F32 ? STEPS : 1];
+    // state
+    f4 o[EV];
+    float m, l;
+
+    __device__ __forceinline__ KvWave(const KvAttend &args) : a(args), lane(threadIdx.x & 63), g((threadIdx.x & 63) >> 4), n(threadIdx.x & 15) {}
+
+    // table entries of the block at p0 (the wave's, or this lane's for its K and V rows)
+    struct Ids {
+        int k, v;
+    };
+    __device__ __forceinline__ int kkey(int t) const { return (n >> 2) * K::GK + t * 4 + (n & 3); }
+    __device__ __forceinline__ Ids ids(int p0) const {
+        if constexpr (PG == 32) {
+            const int i = row[__builtin_amdgcn_readfirstlane((int)page_of(a.c.div, (uint32_t)p0))];
+            return {i, i};
+        } else if constexpr (PG == 8) {
+            const int last = len - 1;
+            return {row[page_of(a.c.div, (uint32_t)min(p0 + (n >> 2) * K::GK, last))], row[page_of(a.c.div, (uint32_t)min(p0 + g * K::GK, last))]};
+        } else {
+            const int i = row[page_of(a.c.div, (uint32_t)min(p0 + (lane & (K::KB - 1)), len - 1))];
+            return {i, i};
+        }
+    }
+    __device__ __forceinline__ int checked(int page, bool *wrong) const {
+        const bool w = (uint32_t)page >= (uint32_t)a.c.n_pages;
+        *wrong |= w;
+        return w ? 0 : page;
+    }
+    __device__ __forceinline__ void place(int p0, Ids id, Spot &s) {
+        if constexpr (PG == 32) {
+            const int page = checked(__builtin_amdgcn_readfirstlane(id.k), &bad);
+            const int slot = p0 - (int)(page_of(a.c.div, (uint32_t)p0) * a.c.div.d);
+            s.k[0] = (page * a.k.page + h * a.k.head + slot * a.k.slot) * ITEM;
+            s.v[0] = (page * a.v.page + h * a.v.head + slot * a.v.slot) * ITEM;
+            s.e[0] = ((int64_t)page * a.c.n_heads + h) * a.c.page_size + slot;
+        } else if constexpr (PG == 8) {
+            const int pk = min(p0 + (n >> 2) * K::GK, (len - 1) & -K::GK), pv = min(p0 + g * K::GK, (len - 1) & -K::GK);
+            const int page_k = checked(id.k, &bad), page_v = checked(id.v, &bad);
+            const int slot_k = pk - (int)(page_of(a.c.div, (uint32_t)pk) * a.c.div.d) + (n & 3);
+            const int slot_v = pv - (int)(page_of(a.c.div, (uint32_t)pv) * a.c.div.d);
+            s.k[0] = (page_k * a.k.page + h * a.k.head + slot_k * a.k.slot + kv_d<CT, HD>(0, g)) * ITEM;
+            s.v[0] = (page_v * a.v.page + h * a.v.head + slot_v * a.v.slot + n * EV) * ITEM;
+            s.e[0] = ((int64_t)page_v * a.c.n_heads + h) * a.c.page_size + slot_v;
+        } else {
+            const int p = min(p0 + (lane & (K::KB - 1)), len - 1);
+            const int page = checked(id.k, &bad);
+            const int slot = p - (int)(page_of(a.c.div, (uint32_t)p) * a.c.div.d);
+            const int64_t kk = (page * a.k.page + h * a.k.head + slot * a.k.slot) * ITEM, vv = (page * a.v.page + h * a.v.head + slot * a.v.slot) * ITEM;
+            const int64_t ee = ((int64_t)page * a.c.n_heads + h) * a.c.page_size + slot;
+#pragma unroll
+            for (int t = 0; t < K::NT; ++t) s.k[t] = shfl64(kk, kkey(t)) + kv_d<CT, HD>(0, g) * ITEM;
+#pragma unroll
+            for (int j = 0; j < K::GK; ++j) {
+                s.v[j] = shfl64(vv, g * K::GK + j) + n * EV * ITEM;
+                if constexpr (K::E4M3) s.e[j] = shfl64(ee, g * K::GK + j);
+            }
+        }
+    }
+    static __device__ __forceinline__ int64_t shfl64(int64_t v, int src) {
+        const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)v, src, 64), hi = (uint32_t)__shfl((int)(uint32_t)(v >> 32), src, 64);
+        return (int64_t)((uint64_t)hi << 32 | lo);
+    }
+
+    __device__ __forceinline__ void fetch(Frag &f, const Spot &s) const {
+        const char *kp = static_cast<const char *>(a.k.p), *vp = static_cast<const char *>(a.v.p);
+#pragma unroll
+        for (int t = 0; t < K::NT; ++t) {
+            const char *r;
+            if constexpr (PG == 32) r = kp + s.k[0] + (uint32_t)(koff + t * 4 * (uint32_t)a.k.slot * ITEM);
+            else if constexpr (PG == 8) r = kp + s.k[0] + t * 4 * a.k.slot * ITEM;
+            else r = kp + s.k[t];
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                const char *p = r + (kv_d<CT, HD>(st, 0) - kv_d<CT, HD>(0, 0)) * ITEM;
+                constexpr int PAIRED = HD / 64 * 2;   // 8-bit pages: steps that share a load
+                if constexpr (!K::E4M3) kv_fetch<16>(f.k[t][st], p);
+                else if (st < PAIRED) {
+                    if (st & 1) continue;
+                    uint32_t w[4];
+                    kv_fetch<16>(w, p);
+                    f.k[t][st][0] = w[0], f.k[t][st][1] = w[1], f.k[t][st + 1][0] = w[2], f.k[t][st + 1][1] = w[3];
+                } else   // (behind the last full 64 the lane groups are 8 apart instead of 16)
+                    kv_fetch<8>(f.k[t][st], p + (kv_d<CT, HD>(st, g) - kv_d<CT, HD>(st, 0) - kv_d<CT, HD>(0, g)) * ITEM);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < K::GK; ++j) {
+            const char *r;
+            if constexpr (PG == 32) r = vp + s.v[0] + (uint32_t)(voff + j * (uint32_t)a.v.slot * ITEM);
+            else if constexpr (PG == 8) r = vp + s.v[0] + j * a.v.slot * ITEM;
+            else r = vp + s.v[j];
+            kv_fetch<EV * ITEM>(f.v[j], r);
+        }
+        if constexpr (K::E4M3) {
+            if constexpr (PG == 1) {
+                uint32_t w[2][2] = {{0, 0}, {0, 0}};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[0][j / 4] |= (uint32_t)a.k.e[s.e[j]] << (j % 4 * 8), w[1][j / 4] |= (uint32_t)a.v.e[s.e[j]] << (j % 4 * 8);
+                f.ke = {w[0][0], w[0][1]}, f.ve = {w[1][0], w[1][1]};
+            } else {
+                const int64_t e = s.e[0] + (PG == 32 ? g * 8 : 0);
+                f.ke = *reinterpret_cast<const uint2 *>(a.k.e + e), f.ve = *reinterpret_cast<const uint2 *>(a.v.e + e);
+            }
+        }
+    }
+
+    static __device__ __forceinline__ f4 mma(u4 x, u4 y, f4 c) {
+        if constexpr (K::F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, x), __builtin_bit_cast(bf8, y), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t codes(uint32_t w, bool high) {   // two 8-bit codes as bf16
+        return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, true))
+                    : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, false));
+    }
+    static __device__ __forceinline__ uint32_t pack16(float x, float y) {
+        const fl2 v = {x, y};
+        if constexpr (K::F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
+        else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf2));
+    }
+    static __device__ __forceinline__ float low16(uint32_t w) {
+        if constexpr (K::F16) return (float)__builtin_bit_cast(h2, w).x;
+        else return __uint_as_float(w << 16);
+    }
+    static __device__ __forceinline__ float high16(uint32_t w) {
+        if constexpr (K::F16) return (float)__builtin_bit_cast(h2, w).y;
+        else return __uint_as_float(w & 0xffff0000u);
+    }
+
+    // One block of KB keys.  Scores as (keys x queries) tiles: A rows are keys, chosen so that lane group g gets keys g * GK
+    // ... + GK - 1 of its query (column n) in order; they are, without leaving the lane, the B operand of (values^T x
+    // weights), whose contraction slots are numbered alike.
+    __device__ __forceinline__ void block(Frag &f, int p0) {
+        constexpr int GK = K::GK;
+        float x[GK];
+#pragma unroll
+        for (int t = 0; t < K::NT; ++t) {
+            f4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                if constexpr (K::F32) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.k[t][st][i]), qf[st][i], s, 0, 0, 0);
+                } else {
+                    u4 w;
+                    if constexpr (K::E4M3)
+                        w = u4{codes(f.k[t][st][0], false), codes(f.k[t][st][0], true), codes(f.k[t][st][1], false), codes(f.k[t][st][1], true)};
+                    else w = u4{f.k[t][st][0], f.k[t][st][1], f.k[t][st][2], f.k[t][st][3]};
+#pragma unroll
+                    for (int p = K::QP - 1; p >= 0; --p) s = mma(w, q[p][st], s);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[t * 4 + r] = s[r];
+        }
+        if constexpr (K::E4M3) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= exp_of((j < 4 ? f.ke.x : f.ke.y) >> (j % 4 * 8) & 255u);
+        }
+#pragma unroll
+        for (int j = 0; j < GK; ++j) x[j] *= a.scale;
+        uint32_t off = 0;   // keys of this lane group behind the end
+        if (p0 + K::KB > len) {
+#pragma unroll
+            for (int j = 0; j < GK; ++j)
+                if (p0 + g * GK + j >= len) {
+                    off |= 1u << j;
+                    x[j] = -__builtin_inff();
+#pragma unroll
+                    for (int i = 0; i < Frag::VD; ++i) f.v[j][i] = 0;
+                }
+        }
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < GK; ++j) top = fmaxf(top, x[j]);
+        if (__any(top > m + (K::BIAS + K::SLACK))) {   // rare once the maximum is found: the reference moves, all sums with it
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float mn = fmaxf(m, top - K::BIAS), c = __builtin_amdgcn_exp2f((m - mn) * KV_LOG2E);
+            m = mn;
+            l *= c;
+#pragma unroll
+            for (int i = 0; i < EV; ++i) o[i] *= c;
+        }
+        float p[GK];
+#pragma unroll
+        for (int j = 0; j < GK; ++j) p[j] = __builtin_amdgcn_exp2f((x[j] - m) * KV_LOG2E);
+#pragma unroll
+        for (int j = 0; j < GK; ++j) l += p[j];
+        if constexpr (K::E4M3) {   // the value's power of two goes into its weight
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float e = exp_of((j < 4 ? f.ve.x : f.ve.y) >> (j % 4 * 8) & 255u);
+                p[j] *= off >> j & 1 ? 0.f : e;
+            }
+        }
+        if constexpr (K::F32) {
+#pragma unroll
+            for (int j = 0; j < GK; ++j)
+#pragma unroll
+                for (int i = 0; i < EV; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[j][i]), p[j], o[i], 0, 0, 0);
+        } else {
+            // a weight is the sum of two 16-bit numbers: with one alone the result is off by up to 2^-9 (bf16) where few keys
+            // share the weight; with both by less than 2^-16
+            u4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                hi[i] = pack16(p[2 * i], p[2 * i + 1]);
+                lo[i] = pack16(p[2 * i] - low16(hi[i]), p[2 * i + 1] - high16(hi[i]));
+            }
+            // values arrive as rows (key j: EV neighbouring columns a lane) and are needed as columns: pairs of rows are
+            // interleaved by byte permutes
+            uint32_t w[8][EV / 2];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < EV / 2; ++i) {
+                    if constexpr (K::E4M3) w[j][i] = codes(f.v[j][i / 2], i & 1);
+                    else w[j][i] = f.v[j][i];
+                }
+#pragma unroll
+            for (int i = 0; i < EV; ++i) {
+                u4 vt;
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj)
+                    vt[jj] = __builtin_amdgcn_perm(w[2 * jj + 1][i / 2], w[2 * jj][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                o[i] = mma(vt, lo, o[i]);
+                o[i] = mma(vt, hi, o[i]);
+            }
+        }
+    }
+
+    __device__ __forceinline__ void load_queries(int s, int hq0, int rows) {
+        const T *src = static_cast<const T *>(a.q) + s * a.q_row + (hq0 + min(n, rows - 1)) * a.q_head;
+        const bool in = n < rows;
+        constexpr int E = K::F32 ? 4 : 8;
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            T raw[E];
+            const int d = kv_d<CT, HD>(st, g);
+            if (a.q_aligned) {
+                const Pack<T, E> p = *reinterpret_cast<const Pack<T, E> *>(src + d);
+#pragma unroll
+                for (int i = 0; i < E; ++i) raw[i] = p.v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) raw[i] = src[d + i];
+            }
+            float v[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] = in ? to_f(raw[i]) : 0.f;
+            if constexpr (K::F32) {
+                qf[st] = f4{v[0], v[1], v[2], v[3]};
+            } else {
+#pragma unroll
+                for (int p = 0; p < K::QP; ++p)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t w = pack16(v[2 * i], v[2 * i + 1]);
+                        q[p][st][i] = w;
+                        v[2 * i] -= low16(w), v[2 * i + 1] -= high16(w);
+                    }
+            }
+        }
+    }
+
+    // blocks b, b + NW, ... < end of this sequence and head; two sets of registers, the next block's loads always in flight
+    __device__ __forceinline__ void run(int b, int end) {
+        m = KV_LOWEST, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < EV; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
+        if (b >= end) return;
+        if constexpr (PG == 32) {
+            koff = (uint32_t)(kkey(0) * (uint32_t)a.k.slot + kv_d<CT, HD>(0, g)) * ITEM;
+            voff = (uint32_t)(g * K::GK * (uint32_t)a.v.slot + n * EV) * ITEM;
+        }
+        Frag f[2];
+        Spot sp;
+        // (a block behind the last one is the last one again: its loads hit the cache and its numbers are not used)
+        const auto next = [&](int x) { return x + NW < end ? x + NW : x; };
+        Ids id = ids(b * K::KB);
+        place(b * K::KB, id, sp);
+        int nb = next(b);
+        id = ids(nb * K::KB);
+        fetch(f[0], sp);
+        while (true) {
+            place(nb * K::KB, id, sp);
+            int n2 = next(nb);
+            id = ids(n2 * K::KB);
+            fetch(f[1], sp);
+            block(f[0], b * K::KB);
+            if (nb == b) break;
+            b = nb, nb = n2;
+            place(nb * K::KB, id, sp);
+            n2 = next(nb);
+            id = ids(n2 * K::KB);
+            fetch(f[0], sp);
+            block(f[1], b * K::KB);
+            if (nb == b) break;
+            b = nb, nb = n2;
+        }
+    }
+};
+
+// One workgroup's part of one (sequence, key head, query tile): blocks [b0, b1).  What the waves found is joined in LDS and
+// goes out as the result, or as a partial one (slot >= 0).
+template <typename CT, typename T, int HD, int PG, int NW>
+__device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW> &w, const KvAttend &a, float *lds, int s, int pair, int len, bool bad_len,
+                                           int b0, int b1, int slot) {
+    constexpr int EV = HD / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = pair / a.q_tiles, qt = pair % a.q_tiles;
+    const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
+    w.row = a.t.t + s * a.t.stride;
+    w.len = len;
+    w.h = h;
+    w.bad = bad_len;
+    w.load_queries(s, hq0, rows);
+    w.run(b0 + wave, b1);
+    if (__any(w.bad)) w.l = __builtin_nanf("");
+    float *lm = lds, *ll = lds + NW * 16, *lo = lds + NW * 32;
+    float l = w.l;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (w.lane < 16) lm[wave * 16 + w.n] = w.m, ll[wave * 16 + w.n] = l;
+    if (w.n < rows) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < EV; ++i) lo[(wave * rows + w.n) * HD + (4 * w.g + r) * EV + i] = w.o[i][r];
+    }
+    __syncthreads();
+    float *part = slot >= 0 ? a.partials + (int64_t)slot * (32 + 16 * HD) : nullptr;
+    for (int e = threadIdx.x; e < rows * HD; e += NW * 64) {
+        const int r = e / HD, d = e % HD;
+        float mm = lm[r];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) mm = fmaxf(mm, lm[i * 16 + r]);
+        float acc = 0.f, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const float c = __builtin_amdgcn_exp2f((lm[i * 16 + r] - mm) * KV_LOG2E);
+            acc = fmaf(lo[(i * rows + r) * HD + d], c, acc);
+            sum = fmaf(ll[i * 16 + r], c, sum);
+        }
+        if (part) {
+            part[32 + e] = acc;
+            if (d == 0) part[r] = mm, part[16 + r] = sum;
+        } else {
+            const bool empty = len == 0 && !bad_len;
+            static_cast<T *>(a.out)[s * a.o_row + (hq0 + r) * a.o_head + d] = from_f<T>(empty ? 0.f : acc / sum);
+            if (a.lse && d == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + r] = empty ? -__builtin_inff() : mm + logf(sum);
+        }
+    }
+}
+
+// The last workgroup of a pair to arrive joins its partial results, in their order.
+template <typename T, int HD, int NW>
+__device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, int pair, int first_wg, int n_parts) {
+    __threadfence();   // every wave's stores are out before the count
+    __syncthreads();   // (and lds is free)
+    int *last = reinterpret_cast<int *>(lds);
+    if (threadIdx.x == 0) {
+        const int before = atomicAdd(&a.counters[first_wg], 1);
+        *last = before == n_parts - 1;
+        if (before == n_parts - 1) a.counters[first_wg] = 0;
+    }
+    __syncthreads();
+    if (!*last) return;
+    __threadfence();
+    const int h = pair / a.q_tiles, qt = pair % a.q_tiles;
+    const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
+    constexpr int64_t SLOT = 32 + 16 * HD;
+    // the first part stands in the slot of a segment that goes on, the others in that of one that came from before
+    const float *p0 = a.partials + (2 * (int64_t)first_wg + 1) * SLOT, *p1 = a.partials + 2 * (int64_t)(first_wg + 1) * SLOT;
+    for (int e = threadIdx.x; e < rows * HD; e += NW * 64) {
+        const int r = e / HD, d = e % HD;
+        float mm = p0[r], sum = p0[16 + r], acc = p0[32 + e];
+        for (int i = 0; i < n_parts - 1; ++i) {
+            const float *p = p1 + 2 * i * SLOT;
+            const float m = p[r], mn = fmaxf(mm, m);
+            const float c0 = __builtin_amdgcn_exp2f((mm - mn) * KV_LOG2E), c1 = __builtin_amdgcn_exp2f((m - mn) * KV_LOG2E);
+            acc = acc * c0 + p[32 + e] * c1;
+            sum = sum * c0 + p[16 + r] * c1;
+            mm = mn;
+        }
+        static_cast<T *>(a.out)[s * a.o_row + (hq0 + r) * a.o_head + d] = from_f<T>(acc / sum);
+        if (a.lse && d == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + r] = mm + logf(sum);
+    }
+}
+
+template <typename CT, typename T, int HD, int PG, int NW>
+__global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_kernel(const KvAttend a) {
+    extern __shared__ __attribute__((aligned(16))) float kv_lds[];
+    constexpr int KB = KvKind<CT, T>::KB, UNIT = KB * NW;
+    const int lane = threadIdx.x & 63;
+    const int pairs = a.c.n_heads * a.q_tiles;   // of one sequence
+    const int64_t capacity = (int64_t)a.t.width * a.c.page_size;
+    const auto length = [&](int raw, bool *wrong) {   // a length outside of the table counts as zero, its results as NaN
+        *wrong = raw < 0 || raw > capacity;
+        return *wrong ? 0 : raw;
+    };
+    KvWave<CT, T, HD, PG, NW> w(a);
+    if (a.direct) {
+        const int s = blockIdx.x / pairs, pair = blockIdx.x % pairs;
+        bool wrong;
+        const int len = length(a.lengths[s], &wrong);
+        kv_segment<CT, T, HD, PG, NW>(w, a, kv_lds, s, pair, len, wrong, 0, (len + KB - 1) / KB, -1);
+        if (__any(w.bad) && lane == 0) kv_report(a.c.error, wrong ? WT_KV_BAD_POSITION : WT_KV_BAD_PAGE);
+        return;
+    }
+    // All pairs' units (NW blocks of KB keys; one for an empty sequence) stand in a row, sequence by sequence; workgroup i
+    // takes the i-th share of them.
+    const auto units = [&](int s) {
+        bool wrong;
+        const int len = length(a.lengths[s], &wrong);
+        return max(1, (len + UNIT - 1) / UNIT);
+    };
+    int64_t total = 0;
+    for (int s0 = 0; s0 < a.t.n_seqs; s0 += 64) total += s0 + lane < a.t.n_seqs ? units(s0 + lane) : 0;
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+    total *= pairs;
+    const int64_t share = max((int64_t)a.min_share, (total + a.n_wg - 1) / a.n_wg);
+    int64_t u = blockIdx.x * share;
+    const int64_t u_end = min(u + share, total);
+    if (u >= u_end) return;
+    // the sequence u falls into: prefix sums, 64 sequences at a time
+    int s = 0;
+    int64_t before = 0;   // units in front of sequence s
+    for (int s0 = 0; s0 < a.t.n_seqs; s0 += 64) {
+        const int64_t mine = s0 + lane < a.t.n_seqs ? (int64_t)units(s0 + lane) * pairs : 0;
+        int64_t incl = mine;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t x = __shfl_up(incl, o, 64);
+            incl += lane >= o ? x : 0;
+        }
+        const uint64_t above = __ballot(before + incl > u);
+        if (above) {
+            const int first = __ffsll((unsigned long long)above) - 1;
+            s = __builtin_amdgcn_readfirstlane(s0 + first);
+            before += __shfl(incl - mine, first, 64);
+            break;
+        }
+        before += __shfl(incl, 63, 64);
+    }
+    while (u < u_end) {
+        bool wrong;
+        const int len = __builtin_amdgcn_readfirstlane(length(a.lengths[s], &wrong));
+        const int n = max(1, (len + UNIT - 1) / UNIT);
+        const int pair = __builtin_amdgcn_readfirstlane((int)((u - before) / n));
+        const int64_t p0 = before + (int64_t)pair * n;   // the pair's first unit
+        const int from = (int)(u - p0), to = (int)min((int64_t)n, u_end - p0);
+        const bool whole = from == 0 && to == n;
+        const int slot = whole ? -1 : 2 * (int)blockIdx.x + (from == 0 ? 1 : 0);
+        kv_segment<CT, T, HD, PG, NW>(w, a, kv_lds, s, pair, len, wrong, from * NW, min(to * NW, (len + KB - 1) / KB), slot);
+        if (__any(w.bad) && lane == 0) kv_report(a.c.error, wrong ? WT_KV_BAD_POSITION : WT_KV_BAD_PAGE);
+        if (!whole) {
+            const int first_wg = (int)(p0 / share), last_wg = (int)((p0 + n - 1) / share);
+            kv_join<T, HD, NW>(a, kv_lds, s, pair, first_wg, last_wg - first_wg + 1);
+        }
+        __syncthreads();   // lds is free
+        u = p0 + to;
+        if (u >= before + (int64_t)n * pairs) before += (int64_t)n * pairs, ++s;
+    }
+}
+
+template <typename CT, typename T, int HD, int PG>
+static int kv_attend_go(const KvAttend &a, unsigned grid, hipStream_t st) {
+    constexpr int NW = 4;
+    const int rows = a.group < 16 ? a.group : 16;
+    const size_t lds = sizeof(float) * NW * (32 + (size_t)rows * HD);
+    if (lds > 64 * 1024) {
+        static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void *>(kv_attend_kernel<CT, T, HD, PG, NW>),
+                                                           hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        WT_HIP(once);
+    }
+    hipLaunchKernelGGL((kv_attend_kernel<CT, T, HD, PG, NW>), dim3(grid), dim3(NW * 64), lds, st, a);
+    WT_HIP(hipGetLastError());
+    return WT_OK;
+}
+
+// page sizes: see KvSpot
+template <typename CT, typename T, int HD>
+static int kv_attend_pages(const KvAttend &a, unsigned grid, hipStream_t st) {
+    constexpr int GK = KvKind<CT, T>::GK;
+    if (a.c.page_size % 32 == 0) return kv_attend_go<CT, T, HD, 32>(a, grid, st);
+    if (a.c.page_size % GK == 0) return kv_attend_go<CT, T, HD, 8>(a, grid, st);
+    return kv_attend_go<CT, T, HD, 1>(a, grid, st);
+}
+
+template <typename CT, typename T>
+static int kv_attend_widths(const KvAttend &a, unsigned grid, hipStream_t st) {
+    switch (a.c.head_dim) {
+        case 32: return kv_attend_pages<CT, T, 32>(a, grid, st);
+        case 64: return kv_attend_pages<CT, T, 64>(a, grid, st);
+        case 96: return kv_attend_pages<CT, T, 96>(a, grid, st);
+        case 128: return kv_attend_pages<CT, T, 128>(a, grid, st);
+        default: return kv_attend_pages<CT, T, 256>(a, grid, st);
+    }
+}
+
+}  // namespace wt

@@ -67,8 +67,8 @@ class PagedKVCache:
         for name, e in (("k_exp", k_exp), ("v_exp", v_exp)):
             if quantised != (e is not None):
                 raise WtError(f"{name}: a float8_e4m3fn cache has exponents, another has none")
-            if quantised and (e.shape != k.shape[:3] or e.dtype != torch.uint8 or not e.is_contiguous()):
-                raise WtError(f"{name}: contiguous uint8 of shape {tuple(k.shape[:3])}")
+            if quantised and (e.shape != k.shape[:3] or e.dtype != torch.uint8 or not e.is_contiguous() or e.data_ptr() % 16):
+                raise WtError(f"{name}: contiguous uint8 of shape {tuple(k.shape[:3])}, 16-byte aligned")
         if quantised and k_exp.data_ptr() == v_exp.data_ptr():
             raise WtError("k_exp and v_exp are the same memory")
         if k.shape[0] > 2 ** 31 - 1 or k.shape[1] > 65535 or k.shape[2] > 2 ** 31 - 1:
@@ -203,11 +203,26 @@ class PagedKVCache:
         lse = torch.empty((n_seqs, hq), dtype=torch.float32, device=self.device) if return_lse else None
         if n_seqs:
             with _lib.on_device(self.k) as st:
+                ws, ws_bytes = self._captured_workspace(n_seqs, hq, width)
                 rc = self._lib.wt_kv_attend(self._p, q.data_ptr(), dt, q.stride(0), q.stride(1), n_seqs, hq,
                                             self.head_dim ** -0.5 if scale is None else float(scale), tp, ts, width, lp, out.data_ptr(),
-                                            out.stride(0), out.stride(1), lse.data_ptr() if return_lse else None, None, 0, st)
+                                            out.stride(0), out.stride(1), lse.data_ptr() if return_lse else None, _lib._ptr(ws) or None, ws_bytes, st)
             _lib._check(rc, "wt_kv_attend")
         return (out, lse) if return_lse else out
+
+    def _captured_workspace(self, n_seqs, n_q_heads, width):
+        """A call that is being captured has a workspace in its graph's own memory, its counters cleared in every replay: two
+        graphs never share one.  Others use the library's arena of their stream."""
+        if not torch.cuda.is_current_stream_capturing():
+            return None, 0
+        n = self._lib.wt_kv_attend_workspace(self._p, n_seqs, n_q_heads, width)
+        if n < 0:
+            _lib._check(n, "wt_kv_attend_workspace")
+        if n == 0:
+            return None, 0
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        ws[:_lib.WT_KV_WORKSPACE_ZEROED].zero_()
+        return ws, n
 
     def check(self):
         """Waits for the device; raises if a call since the last check met something outside of its range."""
