@@ -96,6 +96,8 @@ struct alignas((sizeof(T) * N & -(sizeof(T) * N)) > 16 ? 16 : sizeof(T) * N & -(
 static_assert(sizeof(Pack<float, 6>) == 24 && sizeof(Pack<uint16_t, 6>) == 12 && sizeof(Pack<uint16_t, 8>) == 16, "no padding");
 
 
+constexpr int KV_WAVES = 4;   // waves of a workgroup of the attention kernel
+
 // arguments of one attention call, as its kernels take them (wt_kv_attend.h)
 struct KvAttend {
     KvRows k, v;
@@ -112,7 +114,7 @@ struct KvAttend {
     bool q_aligned;                  // every row of q starts on 16 bytes
     // schedule
     int direct;                      // one workgroup per (sequence, key head, tile): no workspace
-    int n_wg, min_share;
+    int n_wg, min_share, seg_cost;
     int32_t *counters;               // n_wg, zero between calls
     float *partials;                 // 2 * n_wg slots of (32 + 16 * head_dim)
 };

@@ -1,58 +1,69 @@
 // A paged key-value cache: writing it (plain, or in 8 bits with one power of two per row), reading it back, and the
 // attention of one new token per sequence over it.  Layout and formulas: include/wtalign.h, wt_kv_*.
 #include "wt_kv.h"
+#include <type_traits>
 
 namespace wt {
 
-// ---- writing rows ---------------------------------------------------------------------------------------------------
-// A row (one head of one token) is HD values; LPR lanes take EPL = HD / LPR of them each, so that a lane moves 16 bytes of
-// the source (24 for 96 values).  A workgroup takes RT consecutive rows of the call, slots innermost: the rows of a
-// prompt that share a line of the cache (64-value rows of 8 bits: two a line) are written by one workgroup, and a lane
-// group reads and writes whole 64 ... 256 byte runs on both sides.
-template <typename ST, int HD>
+// ---- writing rows and reading them back -----------------------------------------------------------------------------
+// A row (one head of one token) is HD values; LPR lanes take EPL = HD / LPR of them each, so that a lane moves 16 bytes
+// outside of the cache (24 or 12 where a row is 96 values).  A workgroup takes KV_RT consecutive rows of the call, slots
+// innermost: rows of a prompt that share a line of the cache (64 values of 8 bits: two a line) are written by one
+// workgroup, and every lane group moves whole runs of 64 ... 256 bytes on both sides.  Both directions are bound by memory:
+// a lane finds its row's place once and has KV_HU heads' keys and values in flight.
+template <typename T, int HD>
 struct RowSplit {
-    static constexpr int EPL = HD == 96 ? 6 : 16 / (int)sizeof(ST);
+    static constexpr int EPL = HD == 96 ? 6 : 16 / (int)sizeof(T);
     static constexpr int LPR = HD / EPL;
+    static constexpr int GROUPS = 256 / LPR;                 // lane groups of a workgroup: RPW rows x HPW heads
+    static constexpr int RPW = GROUPS < 16 ? GROUPS : 16;
+    static constexpr int HPW = GROUPS / RPW;
 };
-constexpr int KV_RT = 16;
+constexpr int KV_HU = 4;
 
-template <typename ST, typename CT, int HD>
-__device__ __forceinline__ void kv_store_row(const KvRows &x, const KvDims &c, const ST *src, int64_t off, int64_t eoff, int lane) {
-    constexpr int EPL = RowSplit<ST, HD>::EPL, LPR = RowSplit<ST, HD>::LPR;
-    const Pack<ST, EPL> in = *reinterpret_cast<const Pack<ST, EPL> *>(src + lane * EPL);
-    if constexpr (sizeof(CT) != 1) {
-        *reinterpret_cast<Pack<ST, EPL> *>(static_cast<ST *>(x.p) + off + lane * EPL) = in;
-    } else {
-        float f[EPL];
-        float a = 0.f;
+template <int N>   // N bytes as the widest loads and stores their alignment allows
+struct Bytes {
+    static constexpr int W = N % 16 == 0 ? 16 : N % 8 == 0 ? 8 : N % 4 == 0 ? 4 : 2;
+    typedef uint32_t v4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t v2 __attribute__((ext_vector_type(2)));
+    using Word = std::conditional_t<W == 16, v4, std::conditional_t<W == 8, v2, std::conditional_t<W == 4, uint32_t, uint16_t>>>;
+    Word w[N / W];
+    __device__ __forceinline__ void load(const void *p) {
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-            f[i] = to_f(in.v[i]);
-            const float m = fabsf(f[i]);
-            a = m < __builtin_inff() ? fmaxf(a, m) : a;   // infinities and NaN do not choose the power
-        }
-#pragma unroll
-        for (int o = 1; o < LPR; o <<= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
-        // least E with a <= 448 * 2^(E - 127); 448 = 1.75 * 2^8, so E = exponent - 8, one more where the fraction is over .75
-        const int e = min(max((int)((__float_as_uint(a) + 0x1fffffu) >> 23) - 8, 1), 254);
-        const float inv = __uint_as_float((uint32_t)(254 - e) << 23);   // a power of two: the product is exact
-        Pack<uint8_t, EPL> out;
-#pragma unroll
-        for (int i = 0; i < EPL; i += 2) {
-            const float u = f[i] * inv, v = f[i + 1] * inv;
-            const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(u, v, 0, false);
-            out.v[i] = fabsf(f[i]) < __builtin_inff() ? (uint8_t)w : 0x7f;
-            out.v[i + 1] = fabsf(f[i + 1]) < __builtin_inff() ? (uint8_t)(w >> 8) : 0x7f;
-        }
-        uint8_t *dst = static_cast<uint8_t *>(x.p) + off + lane * EPL;
-        if constexpr (EPL == 8) *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(out.v);
-        else if constexpr (EPL == 4) *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(out.v);
-        else {
-#pragma unroll
-            for (int i = 0; i < EPL; i += 2) *reinterpret_cast<uint16_t *>(dst + i) = *reinterpret_cast<const uint16_t *>(out.v + i);
-        }
-        if (lane == 0) x.e[eoff] = (uint8_t)e;
+        for (int i = 0; i < N / W; ++i) w[i] = __builtin_nontemporal_load(static_cast<const Word *>(p) + i);
     }
+    __device__ __forceinline__ void store(void *p) const {
+#pragma unroll
+        for (int i = 0; i < N / W; ++i) __builtin_nontemporal_store(w[i], static_cast<Word *>(p) + i);
+    }
+};
+
+template <typename ST, int EPL, int LPR>
+__device__ __forceinline__ void kv_quantise(const Bytes<EPL * sizeof(ST)> &src, Bytes<EPL> &dst, int *exponent) {
+    ST in[EPL];
+    __builtin_memcpy(in, &src, sizeof(in));
+    float f[EPL];
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+        f[i] = to_f(in[i]);
+        const float m = fabsf(f[i]);
+        a = m < __builtin_inff() ? fmaxf(a, m) : a;   // infinities and NaN do not choose the power
+    }
+#pragma unroll
+    for (int o = 1; o < LPR; o <<= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+    // least E with a <= 448 * 2^(E - 127); 448 = 1.75 * 2^8, so E = exponent - 8, one more where the fraction is over .75
+    const int e = min(max((int)((__float_as_uint(a) + 0x1fffffu) >> 23) - 8, 1), 254);
+    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);   // a power of two: the product is exact
+    uint8_t out[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; i += 2) {
+        const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[i] * inv, f[i + 1] * inv, 0, false);
+        out[i] = fabsf(f[i]) < __builtin_inff() ? (uint8_t)w : 0x7f;
+        out[i + 1] = fabsf(f[i + 1]) < __builtin_inff() ? (uint8_t)(w >> 8) : 0x7f;
+    }
+    __builtin_memcpy(&dst, out, EPL);
+    *exponent = e;
 }
 
 template <typename ST, typename CT, int HD>
@@ -60,65 +71,98 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvRows k, KvRows v, KvDi
                                                         const ST *__restrict__ vs, int64_t k_row, int64_t k_head, int64_t v_row,
                                                         int64_t v_head, int n_rows, const int32_t *__restrict__ sequences,
                                                         const int32_t *__restrict__ positions) {
-    constexpr int LPR = RowSplit<ST, HD>::LPR, HPW = 256 / LPR / KV_RT < 1 ? 1 : 256 / LPR / KV_RT, RPW = 256 / LPR / HPW;
-    const int g = threadIdx.x / LPR, lane = threadIdx.x % LPR;
-    const int h = blockIdx.y * HPW + g / RPW;
-    const int r = blockIdx.x * RPW + g % RPW;
-    if (r >= n_rows || h >= c.n_heads) return;   // whole lane groups
+    using R = RowSplit<ST, HD>;
+    constexpr int EPL = R::EPL;
+    const int g = threadIdx.x / R::LPR, lane = threadIdx.x % R::LPR;
+    const int r = blockIdx.x * R::RPW + g % R::RPW, h0 = blockIdx.y * R::HPW * KV_HU + g / R::RPW;
+    if (g >= R::GROUPS || r >= n_rows) return;   // whole lane groups
     const int pos = positions[r];
-    if (pos < 0) return;
+    Bytes<EPL * sizeof(ST)> kr[KV_HU], vr[KV_HU];
+#pragma unroll
+    for (int i = 0; i < KV_HU; ++i) {   // (beside the look-up of the place)
+        const int h = min(h0 + i * R::HPW, c.n_heads - 1);
+        kr[i].load(ks + r * k_row + h * k_head + lane * EPL);
+        vr[i].load(vs + r * v_row + h * v_head + lane * EPL);
+    }
     int page, slot;
-    if (!kv_place(c, t, sequences ? sequences[r] : r, pos, &page, &slot)) return;
-    const int64_t eoff = ((int64_t)page * c.n_heads + h) * c.page_size + slot;
-    kv_store_row<ST, CT, HD>(k, c, ks + r * k_row + h * k_head, page * k.page + h * k.head + slot * k.slot, eoff, lane);
-    kv_store_row<ST, CT, HD>(v, c, vs + r * v_row + h * v_head, page * v.page + h * v.head + slot * v.slot, eoff, lane);
+    if (pos < 0 || !kv_place(c, t, sequences ? sequences[r] : r, pos, &page, &slot)) return;
+#pragma unroll
+    for (int i = 0; i < KV_HU; ++i) {
+        const int h = h0 + i * R::HPW;
+        if (h >= c.n_heads) break;
+        CT *kd = static_cast<CT *>(k.p) + (page * k.page + h * k.head + slot * k.slot + lane * EPL);
+        CT *vd = static_cast<CT *>(v.p) + (page * v.page + h * v.head + slot * v.slot + lane * EPL);
+        if constexpr (sizeof(CT) != 1) {
+            kr[i].store(kd), vr[i].store(vd);
+        } else {
+            Bytes<EPL> out;
+            int ke, ve;
+            kv_quantise<ST, EPL, R::LPR>(kr[i], out, &ke);
+            out.store(kd);
+            kv_quantise<ST, EPL, R::LPR>(vr[i], out, &ve);
+            out.store(vd);
+            const int64_t eoff = ((int64_t)page * c.n_heads + h) * c.page_size + slot;
+            if (lane == 0) k.e[eoff] = (uint8_t)ke, v.e[eoff] = (uint8_t)ve;
+        }
+    }
 }
 
-// ---- reading rows back ----------------------------------------------------------------------------------------------
-template <typename DT, typename CT, int HD>
-__device__ __forceinline__ void kv_load_row(const KvRows &x, DT *dst, int64_t off, int64_t eoff, bool ok, float fill, int lane) {
-    constexpr int EPL = RowSplit<DT, HD>::EPL;
-    Pack<DT, EPL> out;
-    if (!ok) {
+template <typename DT, typename CT, int EPL>
+__device__ __forceinline__ void kv_emit(const Bytes<EPL * sizeof(CT)> &src, uint32_t e, bool ok, float fill, DT *dst) {
+    Bytes<EPL * sizeof(DT)> out;
+    if constexpr (sizeof(CT) != 1) out = src;
+    if (sizeof(CT) == 1 || !ok) {
+        DT val[EPL];
+        if constexpr (sizeof(CT) == 1) {
+            uint8_t b[EPL];
+            __builtin_memcpy(b, &src, EPL);
+            const float f = exp_of(e);
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) out.v[i] = from_f<DT>(fill);
-    } else if constexpr (sizeof(CT) != 1) {
-        out = *reinterpret_cast<const Pack<DT, EPL> *>(static_cast<const DT *>(x.p) + off + lane * EPL);
-    } else {
-        const float f = exp_of(x.e[eoff]);
-        const uint8_t *src = static_cast<const uint8_t *>(x.p) + off + lane * EPL;
-        uint32_t w[(EPL + 3) / 4];
-        if constexpr (EPL == 8) {
-            const uint2 u = *reinterpret_cast<const uint2 *>(src);
-            w[0] = u.x, w[1] = u.y;
-        } else if constexpr (EPL == 4) w[0] = *reinterpret_cast<const uint32_t *>(src);
-        else {
-            const uint16_t *s = reinterpret_cast<const uint16_t *>(src);
-            w[0] = s[0] | (uint32_t)s[1] << 16, w[1] = s[2];
+            for (int i = 0; i < EPL; ++i) val[i] = from_f<DT>(to_f(fp8_t{b[i]}) * f);
         }
+        if (!ok)
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) out.v[i] = from_f<DT>(to_f(fp8_t{(uint8_t)(w[i / 4] >> (i % 4 * 8))}) * f);
+            for (int i = 0; i < EPL; ++i) val[i] = from_f<DT>(fill);
+        __builtin_memcpy(&out, val, sizeof(out));
     }
-    *reinterpret_cast<Pack<DT, EPL> *>(dst + lane * EPL) = out;
+    out.store(dst);
 }
 
 template <typename DT, typename CT, int HD>
 __global__ __launch_bounds__(256) void kv_gather_kernel(KvRows k, KvRows v, KvDims c, KvTable t, DT *__restrict__ kd,
                                                         DT *__restrict__ vd, int n_rows, const int32_t *__restrict__ sequences,
                                                         const int32_t *__restrict__ positions) {
-    constexpr int LPR = RowSplit<DT, HD>::LPR, HPW = 256 / LPR / KV_RT < 1 ? 1 : 256 / LPR / KV_RT, RPW = 256 / LPR / HPW;
-    const int g = threadIdx.x / LPR, lane = threadIdx.x % LPR;
-    const int h = blockIdx.y * HPW + g / RPW;
-    const int r = blockIdx.x * RPW + g % RPW;
-    if (r >= n_rows || h >= c.n_heads) return;
+    using R = RowSplit<DT, HD>;
+    constexpr int EPL = R::EPL;
+    const int g = threadIdx.x / R::LPR, lane = threadIdx.x % R::LPR;
+    const int r = blockIdx.x * R::RPW + g % R::RPW, h0 = blockIdx.y * R::HPW * KV_HU + g / R::RPW;
+    if (g >= R::GROUPS || r >= n_rows) return;
     const int pos = positions[r];
     int page = 0, slot = 0;
     const bool ok = pos >= 0 && kv_place(c, t, sequences ? sequences[r] : r, pos, &page, &slot);
+    if (!ok) page = 0, slot = 0;   // (a row of the cache all the same: read, not used)
     const float fill = pos < 0 ? 0.f : __builtin_nanf("");
-    const int64_t eoff = ((int64_t)page * c.n_heads + h) * c.page_size + slot;
-    const int64_t to = ((int64_t)r * c.n_heads + h) * HD;
-    kv_load_row<DT, CT, HD>(k, kd + to, page * k.page + h * k.head + slot * k.slot, eoff, ok, fill, lane);
-    kv_load_row<DT, CT, HD>(v, vd + to, page * v.page + h * v.head + slot * v.slot, eoff, ok, fill, lane);
+    Bytes<EPL * sizeof(CT)> kr[KV_HU], vr[KV_HU];
+    uint32_t ke[KV_HU], ve[KV_HU];
+#pragma unroll
+    for (int i = 0; i < KV_HU; ++i) {
+        const int h = min(h0 + i * R::HPW, c.n_heads - 1);
+        kr[i].load(static_cast<const CT *>(k.p) + (page * k.page + h * k.head + slot * k.slot + lane * EPL));
+        vr[i].load(static_cast<const CT *>(v.p) + (page * v.page + h * v.head + slot * v.slot + lane * EPL));
+        if constexpr (sizeof(CT) == 1) {
+            const int64_t eoff = ((int64_t)page * c.n_heads + h) * c.page_size + slot;
+            ke[i] = k.e[eoff], ve[i] = v.e[eoff];
+        } else
+            ke[i] = ve[i] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < KV_HU; ++i) {
+        const int h = h0 + i * R::HPW;
+        if (h >= c.n_heads) break;
+        const int64_t to = ((int64_t)r * c.n_heads + h) * HD + lane * EPL;
+        kv_emit<DT, CT, EPL>(kr[i], ke[i], ok, fill, kd + to);
+        kv_emit<DT, CT, EPL>(vr[i], ve[i], ok, fill, vd + to);
+    }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
@@ -202,10 +246,10 @@ static int kv_check_rows(const char *what, const void *k, const void *v, int n_r
     else if (dtype == WT_DTYPE_F16) M(F, f16_t, f16_t)         \
     else M(F, bf16_t, bf16_t)
 
-template <typename ST, int HD>
+template <typename T, int HD>
 static dim3 kv_row_grid(int n_rows, int n_heads) {
-    constexpr int LPR = RowSplit<ST, HD>::LPR, HPW = 256 / LPR / KV_RT < 1 ? 1 : 256 / LPR / KV_RT, RPW = 256 / LPR / HPW;
-    return dim3((unsigned)((n_rows + RPW - 1) / RPW), (unsigned)((n_heads + HPW - 1) / HPW));
+    using R = RowSplit<T, HD>;
+    return dim3((unsigned)((n_rows + R::RPW - 1) / R::RPW), (unsigned)((n_heads + R::HPW * KV_HU - 1) / (R::HPW * KV_HU)));
 }
 
 int kv_append(const wt_kv_cache *c, const void *k, const void *v, int dtype, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
@@ -258,7 +302,7 @@ int kv_attend_e4m3_bf16(const KvAttend &, unsigned, hipStream_t);
 __global__ void kv_zero_kernel(int32_t *p) { p[blockIdx.x * 256 + threadIdx.x] = 0; }
 
 struct KvPlan {
-    int direct, n_wg, min_share;
+    int direct, n_wg, min_share, seg_cost;
     unsigned grid;
     int64_t bytes;
 };
@@ -272,11 +316,13 @@ static int kv_plan(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_wi
         WT_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
         if (dev < 16) cus[dev] = n;
     }
-    const int unit = c->dtype == WT_DTYPE_F32 ? 64 : 128, group = n_q_heads / c->n_heads;
+    const int group = n_q_heads / c->n_heads;
     const int64_t pairs = (int64_t)n_seqs * c->n_heads * ((group + 15) / 16);
-    p->n_wg = n * 2 < WT_KV_WORKSPACE_ZEROED / 4 ? n * 2 : WT_KV_WORKSPACE_ZEROED / 4;
+    const int64_t key_bytes = 2ll * c->head_dim * (c->dtype == WT_DTYPE_F32 ? 4 : c->dtype == WT_DTYPE_E4M3 ? 1 : 2);   // and its value's
+    p->n_wg = n < WT_KV_WORKSPACE_ZEROED / 4 ? n : WT_KV_WORKSPACE_ZEROED / 4;
     p->min_share = 4;
-    p->direct = (int64_t)table_width * c->page_size <= (int64_t)p->min_share * unit;
+    p->seg_cost = 2;
+    p->direct = (int64_t)table_width * c->page_size * key_bytes <= 512 * 1024;
     p->grid = p->direct ? (unsigned)pairs : (unsigned)p->n_wg;
     p->bytes = p->direct ? 0 : WT_KV_WORKSPACE_ZEROED + (int64_t)p->n_wg * 2 * (32 + 16 * c->head_dim) * 4;
     return WT_OK;
@@ -345,7 +391,7 @@ int kv_attend(const wt_kv_cache *c, const void *q, int dtype, int64_t q_row, int
     a.n_q_heads = n_q_heads, a.group = n_q_heads / c->n_heads, a.q_tiles = (a.group + 15) / 16;
     a.scale = scale, a.lengths = lengths, a.out = out, a.o_row = o_row, a.o_head = o_head, a.lse = lse;
     a.q_aligned = (((uintptr_t)q | (uint64_t)(q_row * item) | (uint64_t)(q_head * item)) & 15) == 0;
-    a.direct = p.direct, a.n_wg = p.n_wg, a.min_share = p.min_share;
+    a.direct = p.direct, a.n_wg = p.n_wg, a.min_share = p.min_share, a.seg_cost = p.seg_cost;
     a.counters = (int32_t *)workspace;
     a.partials = workspace ? (float *)((char *)workspace + WT_KV_WORKSPACE_ZEROED) : nullptr;
     if (c->dtype == WT_DTYPE_E4M3)

@@ -58,10 +58,17 @@ __device__ __forceinline__ void kv_fetch(uint32_t *dst, const char *src) {
         dst[0] = s[0] | (uint32_t)s[1] << 16, dst[1] = s[2];
     } else if constexpr (N <= 16 || N == 24) {
         constexpr int D = N / 4;
-        using P = Pack<uint32_t, D>;
-        const P p = *reinterpret_cast<const P *>(src);
+        typedef uint32_t V __attribute__((ext_vector_type(D < 2 ? 2 : D)));
+        if constexpr (D == 4 || D == 2) {
+            const V p = __builtin_nontemporal_load(reinterpret_cast<const V *>(src));
 #pragma unroll
-        for (int i = 0; i < D; ++i) dst[i] = p.v[i];
+            for (int i = 0; i < D; ++i) dst[i] = p[i];
+        } else {
+            using P = Pack<uint32_t, D>;
+            const P p = *reinterpret_cast<const P *>(src);
+#pragma unroll
+            for (int i = 0; i < D; ++i) dst[i] = p.v[i];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < N / 16; ++i) kv_fetch<16>(dst + 4 * i, src + 16 * i);
@@ -105,9 +112,10 @@ struct KvWave {
         int k, v;
     };
     __device__ __forceinline__ int kkey(int t) const { return (n >> 2) * K::GK + t * 4 + (n & 3); }
-    __device__ __forceinline__ Ids ids(int p0) const {
+    __device__ __forceinline__ Ids ids(int p0) const { return ids(p0, len); }
+    __device__ __forceinline__ Ids ids(int p0, int len) const {
         if constexpr (PG == 32) {
-            const int i = row[__builtin_amdgcn_readfirstlane((int)page_of(a.c.div, (uint32_t)p0))];
+            const int i = row[__builtin_amdgcn_readfirstlane((int)page_of(a.c.div, (uint32_t)min(p0, len - 1)))];
             return {i, i};
         } else if constexpr (PG == 8) {
             const int last = len - 1;
@@ -325,28 +333,38 @@ struct KvWave {
         }
     }
 
-    __device__ __forceinline__ void load_queries(int s, int hq0, int rows) {
+    // the queries in two steps, so that the first block's loads are on their way before the conversion waits
+    static constexpr int QE = K::F32 ? 4 : 8;
+    struct Raw {
+        Pack<T, QE> p[STEPS];
+    };
+    __device__ __forceinline__ void queries_load(Raw &raw, int s, int hq0, int rows) const {
         const T *src = static_cast<const T *>(a.q) + s * a.q_row + (hq0 + min(n, rows - 1)) * a.q_head;
-        const bool in = n < rows;
-        constexpr int E = K::F32 ? 4 : 8;
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) {
-            T raw[E];
             const int d = kv_d<CT, HD>(st, g);
-            if (a.q_aligned) {
-                const Pack<T, E> p = *reinterpret_cast<const Pack<T, E> *>(src + d);
+            if (a.q_aligned) raw.p[st] = *reinterpret_cast<const Pack<T, QE> *>(src + d);
+            else {
 #pragma unroll
-                for (int i = 0; i < E; ++i) raw[i] = p.v[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < E; ++i) raw[i] = src[d + i];
+                for (int i = 0; i < QE; ++i) raw.p[st].v[i] = src[d + i];
             }
-            float v[E];
+        }
+    }
+    __device__ __forceinline__ void queries_take(const Raw &raw, int rows) {   // columns without a query are zeros
+        const bool in = n < rows;
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = in ? to_f(raw[i]) : 0.f;
+        for (int st = 0; st < STEPS; ++st) {
             if constexpr (K::F32) {
-                qf[st] = f4{v[0], v[1], v[2], v[3]};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) qf[st][i] = in ? raw.p[st].v[i] : 0.f;
+            } else if constexpr (K::QP == 1) {
+                const u4 w = __builtin_bit_cast(u4, raw.p[st]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[0][st][i] = in ? w[i] : 0u;
             } else {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = in ? to_f(raw.p[st].v[i]) : 0.f;
 #pragma unroll
                 for (int p = 0; p < K::QP; ++p)
 #pragma unroll
@@ -359,8 +377,9 @@ struct KvWave {
         }
     }
 
-    // blocks b, b + NW, ... < end of this sequence and head; two sets of registers, the next block's loads always in flight
-    __device__ __forceinline__ void run(int b, int end) {
+    // blocks b, b + NW, ... < end of this sequence and head; two sets of registers, the next block's loads always in
+    // flight.  `first`: table entries of block b, loaded before the length was known (and not clamped to it).
+    __device__ __forceinline__ void run(int b, int end, Ids first, const Raw &raw, int rows) {
         m = KV_LOWEST, l = 0.f;
 #pragma unroll
         for (int i = 0; i < EV; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
@@ -369,15 +388,16 @@ struct KvWave {
             koff = (uint32_t)(kkey(0) * (uint32_t)a.k.slot + kv_d<CT, HD>(0, g)) * ITEM;
             voff = (uint32_t)(g * K::GK * (uint32_t)a.v.slot + n * EV) * ITEM;
         }
-        Frag f[2];
-        Spot sp;
         // (a block behind the last one is the last one again: its loads hit the cache and its numbers are not used)
         const auto next = [&](int x) { return x + NW < end ? x + NW : x; };
-        Ids id = ids(b * K::KB);
-        place(b * K::KB, id, sp);
+        if (PG != 32 && (b + 1) * K::KB > len) first = ids(b * K::KB);
+        Frag f[2];
+        Spot sp;
+        place(b * K::KB, first, sp);
         int nb = next(b);
-        id = ids(nb * K::KB);
+        Ids id = ids(nb * K::KB);
         fetch(f[0], sp);
+        queries_take(raw, rows);
         while (true) {
             place(nb * K::KB, id, sp);
             int n2 = next(nb);
@@ -397,20 +417,43 @@ struct KvWave {
     }
 };
 
+__device__ __forceinline__ int64_t kv_capacity(const KvAttend &a) { return (int64_t)a.t.width * a.c.page_size; }
+__device__ __forceinline__ int kv_length(const KvAttend &a, int raw, bool *wrong) {   // a length outside of the table counts as zero, its results as NaN
+    *wrong = raw < 0 || raw > kv_capacity(a);
+    return *wrong ? 0 : raw;
+}
+__device__ __forceinline__ uint32_t kv_div(uint64_t x, uint64_t y) {   // where the quotient fits 32 bits; the wave's operands
+    return ((x | y) >> 32) == 0 ? (uint32_t)x / (uint32_t)y : (uint32_t)(x / y);
+}
+
+// Partial results travel between workgroups, which may run on different XCDs with an L2 each: stored through to memory and
+// loaded from there.  (Fences of the agent's scope around plain stores write back and invalidate whole L2s.)
+__device__ __forceinline__ void kv_put(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float kv_get(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
 // One workgroup's part of one (sequence, key head, query tile): blocks [b0, b1).  What the waves found is joined in LDS and
-// goes out as the result, or as a partial one (slot >= 0).
-template <typename CT, typename T, int HD, int PG, int NW>
+// goes out as the result, or as a partial one (slot >= 0).  LATE: the length is not known yet (all blocks are meant then):
+// queries and first table entries are loaded beside it.
+template <bool LATE, typename CT, typename T, int HD, int PG, int NW>
 __device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW> &w, const KvAttend &a, float *lds, int s, int pair, int len, bool bad_len,
                                            int b0, int b1, int slot) {
-    constexpr int EV = HD / 16;
+    constexpr int EV = HD / 16, KB = KvKind<CT, T>::KB;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = pair / a.q_tiles, qt = pair % a.q_tiles;
     const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
     w.row = a.t.t + s * a.t.stride;
-    w.len = len;
     w.h = h;
+    typename KvWave<CT, T, HD, PG, NW>::Raw raw;
+    const int late_len = LATE ? a.lengths[s] : 0;
+    const auto first = w.ids((b0 + wave) * KB, LATE ? (int)kv_capacity(a) : max(len, 1));
+    w.queries_load(raw, s, hq0, rows);
+    if constexpr (LATE) {
+        len = __builtin_amdgcn_readfirstlane(kv_length(a, late_len, &bad_len));
+        b1 = (len + KB - 1) / KB;
+    }
+    w.len = len;
     w.bad = bad_len;
-    w.load_queries(s, hq0, rows);
-    w.run(b0 + wave, b1);
+    w.run(b0 + wave, b1, first, raw, rows);
+    if (__any(w.bad) && w.lane == 0) kv_report(a.c.error, bad_len ? WT_KV_BAD_POSITION : WT_KV_BAD_PAGE);
     if (__any(w.bad)) w.l = __builtin_nanf("");
     float *lm = lds, *ll = lds + NW * 16, *lo = lds + NW * 32;
     float l = w.l;
@@ -438,8 +481,8 @@ __device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW> &w, const K
             sum = fmaf(ll[i * 16 + r], c, sum);
         }
         if (part) {
-            part[32 + e] = acc;
-            if (d == 0) part[r] = mm, part[16 + r] = sum;
+            kv_put(part + 32 + e, acc);
+            if (d == 0) kv_put(part + r, mm), kv_put(part + 16 + r, sum);
         } else {
             const bool empty = len == 0 && !bad_len;
             static_cast<T *>(a.out)[s * a.o_row + (hq0 + r) * a.o_head + d] = from_f<T>(empty ? 0.f : acc / sum);
@@ -448,10 +491,12 @@ __device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW> &w, const K
     }
 }
 
-// The last workgroup of a pair to arrive joins its partial results, in their order.
+// The last workgroup of a pair to arrive joins its partial results.  A thread takes four columns of a row, and where there
+// are more threads than that, every LANES-th part; JOIN parts are loaded at a time, in an order that never changes.
+constexpr int KV_JOIN = 8;
 template <typename T, int HD, int NW>
 __device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, int pair, int first_wg, int n_parts) {
-    __threadfence();   // every wave's stores are out before the count
+    wait_vmcnt0();     // every wave's stores are where the others read them before the count
     __syncthreads();   // (and lds is free)
     int *last = reinterpret_cast<int *>(lds);
     if (threadIdx.x == 0) {
@@ -461,25 +506,71 @@ __device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, in
     }
     __syncthreads();
     if (!*last) return;
-    __threadfence();
+    __syncthreads();   // (lds is free again)
     const int h = pair / a.q_tiles, qt = pair % a.q_tiles;
     const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
     constexpr int64_t SLOT = 32 + 16 * HD;
+    constexpr int NTH = NW * 64;
+    const int quads = rows * (HD / 4);
+    const int lanes = min(max(NTH / quads, 1), n_parts);   // threads that share four columns
     // the first part stands in the slot of a segment that goes on, the others in that of one that came from before
-    const float *p0 = a.partials + (2 * (int64_t)first_wg + 1) * SLOT, *p1 = a.partials + 2 * (int64_t)(first_wg + 1) * SLOT;
-    for (int e = threadIdx.x; e < rows * HD; e += NW * 64) {
-        const int r = e / HD, d = e % HD;
-        float mm = p0[r], sum = p0[16 + r], acc = p0[32 + e];
-        for (int i = 0; i < n_parts - 1; ++i) {
-            const float *p = p1 + 2 * i * SLOT;
-            const float m = p[r], mn = fmaxf(mm, m);
-            const float c0 = __builtin_amdgcn_exp2f((mm - mn) * KV_LOG2E), c1 = __builtin_amdgcn_exp2f((m - mn) * KV_LOG2E);
-            acc = acc * c0 + p[32 + e] * c1;
-            sum = sum * c0 + p[16 + r] * c1;
-            mm = mn;
+    const auto part = [&](int i) { return a.partials + (i == 0 ? 2 * (int64_t)first_wg + 1 : 2 * (int64_t)(first_wg + i)) * SLOT; };
+    for (int e0 = 0; e0 < quads; e0 += NTH / lanes) {
+        const int e = e0 + threadIdx.x / lanes, mine = threadIdx.x % lanes;
+        const bool in = e < quads && threadIdx.x / lanes < NTH / lanes;
+        const int r = in ? e / (HD / 4) : 0, d = in ? e % (HD / 4) * 4 : 0;
+        float mm = KV_LOWEST, sum = 0.f;
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = mine; i0 < n_parts; i0 += lanes * KV_JOIN) {
+            float m[KV_JOIN], l[KV_JOIN], o[KV_JOIN][4];
+#pragma unroll
+            for (int i = 0; i < KV_JOIN; ++i) {
+                const bool there = i0 + i * lanes < n_parts;
+                const float *p = part(there ? i0 + i * lanes : i0);
+                m[i] = kv_get(p + r), l[i] = kv_get(p + 16 + r);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[i][x] = kv_get(p + 32 + r * HD + d + x);
+            }
+            float mn = mm;
+#pragma unroll
+            for (int i = 0; i < KV_JOIN; ++i) mn = fmaxf(mn, m[i]);   // (one that stands in for a missing part changes nothing)
+            const float c = __builtin_amdgcn_exp2f((mm - mn) * KV_LOG2E);
+            sum *= c, acc *= c, mm = mn;
+#pragma unroll
+            for (int i = 0; i < KV_JOIN; ++i) {
+                const bool there = i0 + i * lanes < n_parts;
+                const float w = __builtin_amdgcn_exp2f((m[i] - mm) * KV_LOG2E);
+                if (there) {
+                    sum = fmaf(l[i], w, sum);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) acc[x] = fmaf(o[i][x], w, acc[x]);
+                }
+            }
         }
-        static_cast<T *>(a.out)[s * a.o_row + (hq0 + r) * a.o_head + d] = from_f<T>(acc / sum);
-        if (a.lse && d == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + r] = mm + logf(sum);
+        if (lanes > 1) {
+            float *mine_lds = lds + 6 * threadIdx.x;
+            mine_lds[0] = mm, mine_lds[1] = sum;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) mine_lds[2 + x] = acc[x];
+            __syncthreads();
+            if (mine == 0)
+                for (int i = 1; i < lanes; ++i) {
+                    const float *p = mine_lds + 6 * i;
+                    const float mn = fmaxf(mm, p[0]);
+                    const float c0 = __builtin_amdgcn_exp2f((mm - mn) * KV_LOG2E), c1 = __builtin_amdgcn_exp2f((p[0] - mn) * KV_LOG2E);
+                    sum = sum * c0 + p[1] * c1;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) acc[x] = acc[x] * c0 + p[2 + x] * c1;
+                    mm = mn;
+                }
+            __syncthreads();
+        }
+        if (in && mine == 0) {
+            T *dst = static_cast<T *>(a.out) + s * a.o_row + (hq0 + r) * a.o_head + d;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) dst[x] = from_f<T>(acc[x] / sum);
+            if (a.lse && d == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + r] = mm + logf(sum);
+        }
     }
 }
 
@@ -489,80 +580,86 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_kernel(c
     constexpr int KB = KvKind<CT, T>::KB, UNIT = KB * NW;
     const int lane = threadIdx.x & 63;
     const int pairs = a.c.n_heads * a.q_tiles;   // of one sequence
-    const int64_t capacity = (int64_t)a.t.width * a.c.page_size;
-    const auto length = [&](int raw, bool *wrong) {   // a length outside of the table counts as zero, its results as NaN
-        *wrong = raw < 0 || raw > capacity;
-        return *wrong ? 0 : raw;
-    };
     KvWave<CT, T, HD, PG, NW> w(a);
     if (a.direct) {
-        const int s = blockIdx.x / pairs, pair = blockIdx.x % pairs;
-        bool wrong;
-        const int len = length(a.lengths[s], &wrong);
-        kv_segment<CT, T, HD, PG, NW>(w, a, kv_lds, s, pair, len, wrong, 0, (len + KB - 1) / KB, -1);
-        if (__any(w.bad) && lane == 0) kv_report(a.c.error, wrong ? WT_KV_BAD_POSITION : WT_KV_BAD_PAGE);
+        kv_segment<true, CT, T, HD, PG, NW>(w, a, kv_lds, blockIdx.x / pairs, blockIdx.x % pairs, 0, false, 0, 0, -1);
         return;
     }
-    // All pairs' units (NW blocks of KB keys; one for an empty sequence) stand in a row, sequence by sequence; workgroup i
-    // takes the i-th share of them.
-    const auto units = [&](int s) {
-        bool wrong;
-        const int len = length(a.lengths[s], &wrong);
-        return max(1, (len + UNIT - 1) / UNIT);
+    // All pairs stand in a row, sequence by sequence, each with seg_cost units for what a segment costs by itself (queries,
+    // joining the waves) and then one for every NW blocks of keys; workgroup i takes the i-th share of the row.
+    const int n_seqs = a.t.n_seqs, head = a.seg_cost;
+    int raw = 0, base = 0;   // lengths of 64 sequences from `base` on, one a lane
+    const auto load = [&](int s0) {
+        base = s0;
+        raw = a.lengths[min(s0 + lane, n_seqs - 1)];
     };
-    int64_t total = 0;
-    for (int s0 = 0; s0 < a.t.n_seqs; s0 += 64) total += s0 + lane < a.t.n_seqs ? units(s0 + lane) : 0;
+    const auto units = [&](int r) {
+        bool wrong;
+        return (kv_length(a, r, &wrong) + UNIT - 1) / UNIT;
+    };
+    uint64_t total = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+        load(s0);
+        total += s0 + lane < n_seqs ? units(raw) + head : 0;
+    }
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
     total *= pairs;
-    const int64_t share = max((int64_t)a.min_share, (total + a.n_wg - 1) / a.n_wg);
-    int64_t u = blockIdx.x * share;
-    const int64_t u_end = min(u + share, total);
+    total = (uint64_t)__builtin_amdgcn_readfirstlane((int)(total >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
+    const uint32_t share = max((uint32_t)a.min_share, kv_div(total + a.n_wg - 1, a.n_wg));
+    uint64_t u = (uint64_t)blockIdx.x * share;
+    const uint64_t u_end = min(u + share, total);
     if (u >= u_end) return;
     // the sequence u falls into: prefix sums, 64 sequences at a time
     int s = 0;
-    int64_t before = 0;   // units in front of sequence s
-    for (int s0 = 0; s0 < a.t.n_seqs; s0 += 64) {
-        const int64_t mine = s0 + lane < a.t.n_seqs ? (int64_t)units(s0 + lane) * pairs : 0;
-        int64_t incl = mine;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t x = __shfl_up(incl, o, 64);
+    uint64_t before = 0;   // units in front of sequence s
+    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+        if (base != s0) load(s0);
+        const uint64_t mine = s0 + lane < n_seqs ? (uint64_t)(units(raw) + head) * pairs : 0;
+        uint64_t incl = mine;
+        for (int o = 1; o < min(64, n_seqs); o <<= 1) {
+            const uint64_t x = __shfl_up(incl, o, 64);
             incl += lane >= o ? x : 0;
         }
         const uint64_t above = __ballot(before + incl > u);
+        const int first = above ? __ffsll((unsigned long long)above) - 1 : 63;
+        const uint64_t add = __shfl(above ? incl - mine : incl, first, 64);
+        before += (uint64_t)__builtin_amdgcn_readfirstlane((int)(add >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)add);
         if (above) {
-            const int first = __ffsll((unsigned long long)above) - 1;
-            s = __builtin_amdgcn_readfirstlane(s0 + first);
-            before += __shfl(incl - mine, first, 64);
+            s = s0 + first;
             break;
         }
-        before += __shfl(incl, 63, 64);
     }
     while (u < u_end) {
+        if (s >= base + 64) load(base + 64);
         bool wrong;
-        const int len = __builtin_amdgcn_readfirstlane(length(a.lengths[s], &wrong));
-        const int n = max(1, (len + UNIT - 1) / UNIT);
-        const int pair = __builtin_amdgcn_readfirstlane((int)((u - before) / n));
-        const int64_t p0 = before + (int64_t)pair * n;   // the pair's first unit
-        const int from = (int)(u - p0), to = (int)min((int64_t)n, u_end - p0);
-        const bool whole = from == 0 && to == n;
-        const int slot = whole ? -1 : 2 * (int)blockIdx.x + (from == 0 ? 1 : 0);
-        kv_segment<CT, T, HD, PG, NW>(w, a, kv_lds, s, pair, len, wrong, from * NW, min(to * NW, (len + KB - 1) / KB), slot);
-        if (__any(w.bad) && lane == 0) kv_report(a.c.error, wrong ? WT_KV_BAD_POSITION : WT_KV_BAD_PAGE);
-        if (!whole) {
-            const int first_wg = (int)(p0 / share), last_wg = (int)((p0 + n - 1) / share);
-            kv_join<T, HD, NW>(a, kv_lds, s, pair, first_wg, last_wg - first_wg + 1);
+        const int len = kv_length(a, __builtin_amdgcn_readlane(raw, s - base), &wrong);
+        const int n = (len + UNIT - 1) / UNIT, cost = n + head;
+        const int pair = (int)kv_div(u - before, cost);
+        const uint64_t p0 = before + (uint64_t)pair * cost;   // the pair's first unit, and that of its keys
+        const uint64_t k0 = p0 + head;
+        const uint64_t stop = min(p0 + cost, u_end);
+        const int from = u > k0 ? (int)(u - k0) : 0, to = stop > k0 ? (int)(stop - k0) : 0;
+        if (n == 0 ? u == p0 : to > from) {   // (an empty sequence belongs to the workgroup that holds its first unit)
+            const bool whole = from == 0 && to == n;
+            const int slot = whole ? -1 : 2 * (int)blockIdx.x + (from == 0 ? 1 : 0);
+            kv_segment<false, CT, T, HD, PG, NW>(w, a, kv_lds, s, pair, len, wrong, from * NW, min(to * NW, (len + KB - 1) / KB), slot);
+            if (!whole) {
+                const int first_wg = (int)kv_div(k0, share), last_wg = (int)kv_div(k0 + n - 1, share);
+                kv_join<T, HD, NW>(a, kv_lds, s, pair, first_wg, last_wg - first_wg + 1);
+            }
+            __syncthreads();   // lds is free
         }
-        __syncthreads();   // lds is free
-        u = p0 + to;
-        if (u >= before + (int64_t)n * pairs) before += (int64_t)n * pairs, ++s;
+        u = stop;
+        if (u >= before + (uint64_t)cost * pairs) before += (uint64_t)cost * pairs, ++s;
     }
 }
 
 template <typename CT, typename T, int HD, int PG>
 static int kv_attend_go(const KvAttend &a, unsigned grid, hipStream_t st) {
-    constexpr int NW = 4;
+    constexpr int NW = KV_WAVES;
     const int rows = a.group < 16 ? a.group : 16;
-    const size_t lds = sizeof(float) * NW * (32 + (size_t)rows * HD);
+    size_t lds = sizeof(float) * NW * (32 + (size_t)rows * HD);
+    if (lds < sizeof(float) * NW * 64 * 6) lds = sizeof(float) * NW * 64 * 6;   // what the join of partial results takes
     if (lds > 64 * 1024) {
         static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void *>(kv_attend_kernel<CT, T, HD, PG, NW>),
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
@@ -572,7 +669,6 @@ static int kv_attend_go(const KvAttend &a, unsigned grid, hipStream_t st) {
     WT_HIP(hipGetLastError());
     return WT_OK;
 }
-
 // page sizes: see KvSpot
 template <typename CT, typename T, int HD>
 static int kv_attend_pages(const KvAttend &a, unsigned grid, hipStream_t st) {

@@ -28,6 +28,14 @@ from ._lib import WtError
 _DTYPES = {torch.float32: _lib.WT_DTYPE_F32, torch.float16: _lib.WT_DTYPE_F16, torch.bfloat16: _lib.WT_DTYPE_BF16}
 _PAGE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.WT_DTYPE_E4M3}
 HEAD_DIMS = (32, 64, 96, 128, 256)
+_current_device = torch.cuda.current_device
+
+
+def _raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)     # (the same handle, without a Stream object around it)
 
 
 def _overlaps(t):
@@ -80,6 +88,9 @@ class PagedKVCache:
         self.n_pages, self.n_heads, self.page_size, self.head_dim = k.shape
         self.error = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._lib = _lib.load()
+        self._append, self._gather, self._attend = self._lib.wt_kv_append, self._lib.wt_kv_gather, self._lib.wt_kv_attend
+        self._index = self.device.index
+        self._scale = self.head_dim ** -0.5
 
         def strides(t):    # (a dimension of size one has no stride to speak of)
             return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
@@ -98,44 +109,59 @@ class PagedKVCache:
             return cls(k.view(dtype), v.view(dtype), ke, ve)
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
 
-    # --- arguments
+    # --- arguments (a step of a decoder makes two calls a layer: these checks are kept short)
     def _dtype(self, t_dtype, name):
         """An 8-bit cache takes and gives any of the three types, another only its own."""
-        if t_dtype not in _DTYPES or (self.k_exp is None and t_dtype != self.dtype):
+        dt = _DTYPES.get(t_dtype)
+        if dt is None or (self.k_exp is None and t_dtype is not self.dtype):
             raise WtError(f"{name}: {t_dtype} with a cache of {self.dtype}")
-        return _DTYPES[t_dtype]
+        return dt
 
-    def _int32(self, t, name, shape=None):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous() or \
-                (shape is not None and t.shape != shape):
-            raise WtError(f"{name}: contiguous int32 on {self.device}" + (f" of shape {tuple(shape)}" if shape is not None else ""))
+    def _int32(self, t, name, n):
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != self.device or t.dim() != 1 or t.shape[0] != n or \
+                not t.is_contiguous():
+            raise WtError(f"{name}: {n} contiguous int32 on {self.device}")
         return t.data_ptr()
 
     def _table(self, table):
-        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype != torch.int32 or table.device != self.device or \
-                table.shape[1] < 1 or table.stride(1) != 1 or (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
-            raise WtError(f"page table: int32 (sequences, pages) on {self.device}, the pages of a sequence side by side")
+        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype is not torch.int32 or table.device != self.device:
+            raise WtError(f"page table: int32 (sequences, pages) on {self.device}")
         n, width = table.shape
+        stride, one = table.stride()
+        if width < 1 or (one != 1 and width > 1) or (n > 1 and stride < width):
+            raise WtError("page table: the pages of a sequence stand side by side, its rows apart")
         if width * self.page_size > 2 ** 31 - 1:
             raise WtError(f"page table: {width} pages of {self.page_size} are beyond 32-bit positions")
-        return table.data_ptr(), table.stride(0) if n > 1 else width, n, width
+        return table.data_ptr(), stride if n > 1 else width, n, width
 
     def _rows_of(self, positions, sequences, n_seqs):
         if not isinstance(positions, torch.Tensor) or positions.dim() != 1:
             raise WtError("positions: one int32 per row")
         n = positions.shape[0]
-        pos = self._int32(positions, "positions")
+        pos = self._int32(positions, "positions", n)
         if sequences is None and n > n_seqs:
             raise WtError(f"{n} rows for {n_seqs} sequences: say whose they are (sequences=)")
-        return n, None if sequences is None else self._int32(sequences, "sequences", positions.shape), pos
+        return n, None if sequences is None else self._int32(sequences, "sequences", n), pos
 
     def _new(self, t, name, n):
-        if not isinstance(t, torch.Tensor) or t.shape != (n, self.n_heads, self.head_dim) or t.device != self.device:
+        if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.device != self.device or tuple(t.shape) != (n, self.n_heads, self.head_dim):
             raise WtError(f"{name}: ({n}, {self.n_heads}, {self.head_dim}) on {self.device}")
-        item = t.element_size()
-        if n and (t.stride(2) != 1 or t.data_ptr() % 16 or (n > 1 and t.stride(0) * item % 16) or (self.n_heads > 1 and t.stride(1) * item % 16)):
+        row, head, one = t.stride()
+        row, head = row if n > 1 else 0, head if self.n_heads > 1 else 0
+        p, item = t.data_ptr(), t.element_size()
+        if n and (one != 1 or (p | row * item | head * item) & 15):
             raise WtError(f"{name}: rows must be contiguous and start on 16-byte steps (strides {t.stride()})")
-        return t.data_ptr(), t.stride(0) if n > 1 else 0, t.stride(1) if self.n_heads > 1 else 0
+        return p, row, head
+
+    def _call(self, entry, what, *args):
+        """The entry on the current stream of the cache's device."""
+        if _current_device() == self._index:
+            rc = entry(self._p, *args, _raw_stream(self._index))
+        else:
+            with torch.cuda.device(self.device):
+                rc = entry(self._p, *args, _raw_stream(self._index))
+        if rc:
+            _lib._check(rc, what)
 
     # --- operators
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, sequences: torch.Tensor | None = None):
@@ -144,16 +170,13 @@ class PagedKVCache:
         two rows of a call may name the same place."""
         tp, ts, n_seqs, width = self._table(table)
         n, seq, pos = self._rows_of(positions, sequences, n_seqs)
-        if k.dtype != v.dtype:
-            raise WtError(f"k and v differ: {k.dtype}, {v.dtype}")
-        dt = self._dtype(k.dtype, "k, v")
         kp, k_row, k_head = self._new(k, "k", n)
         vp, v_row, v_head = self._new(v, "v", n)
-        if n == 0:
-            return
-        with _lib.on_device(self.k) as st:
-            rc = self._lib.wt_kv_append(self._p, kp, vp, dt, k_row, k_head, v_row, v_head, n, tp, ts, n_seqs, width, seq, pos, st)
-        _lib._check(rc, "wt_kv_append")
+        if k.dtype is not v.dtype:
+            raise WtError(f"k and v differ: {k.dtype}, {v.dtype}")
+        dt = self._dtype(k.dtype, "k, v")
+        if n:
+            self._call(self._append, "wt_kv_append", kp, vp, dt, k_row, k_head, v_row, v_head, n, tp, ts, n_seqs, width, seq, pos)
 
     def gather(self, table: torch.Tensor, positions: torch.Tensor, sequences: torch.Tensor | None = None, dtype=None, out=None):
         """-> (k, v), each (rows, heads, head_dim): the rows at ``positions[r]`` of sequence ``sequences[r]``, in the cache's
@@ -162,67 +185,82 @@ class PagedKVCache:
         tp, ts, n_seqs, width = self._table(table)
         n, seq, pos = self._rows_of(positions, sequences, n_seqs)
         if out is None:
-            dtype = dtype if dtype is not None else (torch.float32 if self.k_exp is not None else self.dtype)
+            if dtype is None:
+                dtype = torch.float32 if self.k_exp is not None else self.dtype
             dt = self._dtype(dtype, "dtype")
-            out = tuple(torch.empty((n, self.n_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
+            k = torch.empty((n, self.n_heads, self.head_dim), dtype=dtype, device=self.device)
+            v = torch.empty_like(k)
+            out = k, v
         else:
             k, v = out
-            if k.dtype != v.dtype or (dtype is not None and k.dtype != dtype):
+            self._new(k, "out[0]", n), self._new(v, "out[1]", n)
+            if k.dtype is not v.dtype or (dtype is not None and k.dtype is not dtype):
                 raise WtError(f"out: {k.dtype} and {v.dtype}" + (f", not {dtype}" if dtype is not None else ""))
             dt = self._dtype(k.dtype, "out")
-            for name, t in (("out[0]", k), ("out[1]", v)):
-                self._new(t, name, n)
-                if not t.is_contiguous():
-                    raise WtError(f"{name}: not contiguous")
+            if not k.is_contiguous() or not v.is_contiguous():
+                raise WtError("out: not contiguous")
             if n and k.data_ptr() == v.data_ptr():
                 raise WtError("out: the same memory twice")
         if n:
-            with _lib.on_device(self.k) as st:
-                rc = self._lib.wt_kv_gather(self._p, out[0].data_ptr(), out[1].data_ptr(), dt, n, tp, ts, n_seqs, width, seq, pos, st)
-            _lib._check(rc, "wt_kv_gather")
+            self._call(self._gather, "wt_kv_gather", k.data_ptr(), v.data_ptr(), dt, n, tp, ts, n_seqs, width, seq, pos)
         return out
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, scale: float | None = None,
-               out: torch.Tensor | None = None, return_lse: bool = False):
+               out: torch.Tensor | None = None, return_lse: bool = False, workspace: torch.Tensor | None = None):
         """One new token of every sequence: q (B, query heads, head_dim) over the sequence's positions 0 ... lengths[b] - 1;
         query head h reads key head h // (query heads // heads).  -> (B, query heads, head_dim) in q's type, with
         ``return_lse`` also the float32 (B, query heads) logarithm of its sum of exponentials.  A length of zero gives
-        zeros (and -inf).  ``scale``: default head_dim ** -0.5.  ``out`` may be q itself."""
+        zeros (and -inf).  ``scale``: default head_dim ** -0.5.  ``out`` may be q itself.
+
+        Long sequences are split over workgroups that meet in a workspace: the library's own of the current stream, or
+        ``workspace`` (from ``attend_workspace``).  Calls that may run at the same time need one each.  A call that is being
+        captured into a graph has none of the stream's: without ``workspace`` it takes one in the graph's memory, which
+        costs every replay a small kernel that clears its counters."""
         tp, ts, n_seqs, width = self._table(table)
-        if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.shape[0] != n_seqs or q.shape[2] != self.head_dim or \
-                q.shape[1] < 1 or q.shape[1] % self.n_heads or q.device != self.device or q.stride(2) != 1:
-            raise WtError(f"q: ({n_seqs}, a multiple of {self.n_heads}, {self.head_dim}) on {self.device}, a head's values side by side")
+        if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.device != self.device:
+            raise WtError(f"q: (sequences, query heads, head_dim) on {self.device}")
+        n, hq, d = q.shape
+        q_row, q_head, one = q.stride()
+        if n != n_seqs or d != self.head_dim or one != 1 or hq < 1 or hq % self.n_heads:
+            raise WtError(f"q: ({n_seqs}, a multiple of {self.n_heads}, {self.head_dim}), a head's values side by side (got {tuple(q.shape)}, "
+                          f"strides {q.stride()})")
         dt = self._dtype(q.dtype, "q")
-        lp = self._int32(lengths, "lengths", (n_seqs,))
+        lp = self._int32(lengths, "lengths", n)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or out.stride(2) != 1 or \
-                _overlaps(out):
-            raise WtError(f"out: {tuple(q.shape)} of {q.dtype} on {self.device}, a head's values side by side, no two in one place")
-        hq = q.shape[1]
-        lse = torch.empty((n_seqs, hq), dtype=torch.float32, device=self.device) if return_lse else None
-        if n_seqs:
-            with _lib.on_device(self.k) as st:
-                ws, ws_bytes = self._captured_workspace(n_seqs, hq, width)
-                rc = self._lib.wt_kv_attend(self._p, q.data_ptr(), dt, q.stride(0), q.stride(1), n_seqs, hq,
-                                            self.head_dim ** -0.5 if scale is None else float(scale), tp, ts, width, lp, out.data_ptr(),
-                                            out.stride(0), out.stride(1), lse.data_ptr() if return_lse else None, _lib._ptr(ws) or None, ws_bytes, st)
-            _lib._check(rc, "wt_kv_attend")
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            o_row, o_head = hq * d, d
+        else:
+            if out.shape != q.shape or out.dtype is not q.dtype or out.device != self.device or out.stride(2) != 1 or _overlaps(out):
+                raise WtError(f"out: {tuple(q.shape)} of {q.dtype} on {self.device}, a head's values side by side, no two in one place")
+            o_row, o_head, _ = out.stride()
+        lse = torch.empty((n, hq), dtype=torch.float32, device=self.device) if return_lse else None
+        if n:
+            wp, w_bytes = None, 0
+            if workspace is not None:
+                if workspace.dtype is not torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
+                    raise WtError("workspace: what attend_workspace() gave")
+                wp, w_bytes = workspace.data_ptr(), workspace.numel()
+            elif torch.cuda.is_current_stream_capturing():
+                workspace = self.attend_workspace(hq, table)
+                if workspace is not None:
+                    wp, w_bytes = workspace.data_ptr(), workspace.numel()
+            self._call(self._attend, "wt_kv_attend", q.data_ptr(), dt, q_row, q_head, n, hq, self._scale if scale is None else scale, tp, ts,
+                       width, lp, out.data_ptr(), o_row, o_head, lse.data_ptr() if return_lse else None, wp, w_bytes)
         return (out, lse) if return_lse else out
 
-    def _captured_workspace(self, n_seqs, n_q_heads, width):
-        """A call that is being captured has a workspace in its graph's own memory, its counters cleared in every replay: two
-        graphs never share one.  Others use the library's arena of their stream."""
-        if not torch.cuda.is_current_stream_capturing():
-            return None, 0
-        n = self._lib.wt_kv_attend_workspace(self._p, n_seqs, n_q_heads, width)
+    def attend_workspace(self, n_q_heads: int, table: torch.Tensor) -> torch.Tensor | None:
+        """A workspace for ``attend`` calls with this many query heads and tables of this shape (or fewer sequences, or fewer
+        pages): made ready once, left ready by every call.  None: such calls need none."""
+        _, _, n_seqs, width = self._table(table)
+        with torch.cuda.device(self.device):
+            n = self._lib.wt_kv_attend_workspace(self._p, n_seqs, n_q_heads, width)
         if n < 0:
             _lib._check(n, "wt_kv_attend_workspace")
         if n == 0:
-            return None, 0
+            return None
         ws = torch.empty(n, dtype=torch.uint8, device=self.device)
         ws[:_lib.WT_KV_WORKSPACE_ZEROED].zero_()
-        return ws, n
+        return ws
 
     def check(self):
         """Waits for the device; raises if a call since the last check met something outside of its range."""
