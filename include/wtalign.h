@@ -44,6 +44,8 @@ extern "C" {
 #define WT_E_UNSUPPORTED (-3) /* shape outside the kernels' range: T > 256 or F > 1792.
                                  The reference never exceeds T <= 226, F <= 1500        */
 
+#define WT_E_CAPTURE (-4)     /* wt_kv_attend on a capturing stream without a workspace of its own */
+
 #define WT_DTYPE_F32 0
 #define WT_DTYPE_F16 1
 
@@ -301,6 +303,8 @@ WT_API int wt_logmel_pad_batch(const float *pcm, int n_chunks, int64_t n_samples
 #define WT_DTYPE_BF16 2
 #define WT_DTYPE_E4M3 3 /* the cache's pages only */
 
+#define WT_KV_MAX_POSITIONS 0x7fffff00 /* most positions that a table's row may name: table_width * page_size               */
+
 #define WT_KV_BAD_POSITION 1 /* a position (append, gather) or a length (attend) outside of the table's row          */
 #define WT_KV_BAD_PAGE 2     /* a table entry in use outside of [0, n_pages)                                            */
 #define WT_KV_BAD_SEQUENCE 4 /* sequences[r] outside of [0, n_seqs)                                                     */
@@ -350,7 +354,7 @@ WT_API int wt_kv_gather(const wt_kv_cache *cache, void *k, void *v, int dtype, i
  *   lse    : optional device fp32 [n_seqs][n_q_heads]
  *   workspace : wt_kv_attend_workspace() bytes of device memory, 16-byte aligned, its first WT_KV_WORKSPACE_ZEROED bytes zeroed
  *            once before its first use; every call leaves it ready for the next one.  Two calls that may run at the same time (on two streams, or in two
- *            graphs) need one each.  NULL: the library's arena of this stream; refused while the stream is capturing */
+ *            graphs) need one each.  NULL: the library's arena of this stream; WT_E_CAPTURE while the stream is capturing */
 WT_API int wt_kv_attend(const wt_kv_cache *cache, const void *q, int dtype, int64_t q_row_stride, int64_t q_head_stride, int n_seqs,
                         int n_q_heads, float scale, const int32_t *table, int64_t table_stride, int table_width,
                         const int32_t *lengths, void *out, int64_t out_row_stride, int64_t out_head_stride, float *lse,

@@ -98,6 +98,8 @@ static_assert(sizeof(Pack<float, 6>) == 24 && sizeof(Pack<uint16_t, 6>) == 12 &&
 
 constexpr int KV_WAVES = 4;   // waves of a workgroup of the attention kernel
 
+constexpr int kv_slot(int head_dim) { return 64 + 16 * head_dim; }   // floats of a partial result
+
 // arguments of one attention call, as its kernels take them (wt_kv_attend.h)
 struct KvAttend {
     KvRows k, v;
@@ -111,12 +113,12 @@ struct KvAttend {
     void *out;
     int64_t o_row, o_head;
     float *lse;
-    bool q_aligned;                  // every row of q starts on 16 bytes
+    bool q_aligned, o_aligned;       // every row of q starts on 16 bytes; of out, on four elements
     // schedule
-    int direct;                      // one workgroup per (sequence, key head, tile): no workspace
+    int direct;                      // 1: one workgroup per (sequence, key head, tile), 2: one wave; no workspace
     int n_wg, min_share, seg_cost;
-    int32_t *counters;               // n_wg, zero between calls
-    float *partials;                 // 2 * n_wg slots of (32 + 16 * head_dim)
+    int32_t *counters;               // 4 * n_wg, zero between calls
+    float *partials;                 // 2 * n_wg slots: maxima and sums of 16 queries, the same of a joined group, sums of values
 };
 
 }  // namespace wt

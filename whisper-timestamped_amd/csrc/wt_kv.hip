@@ -202,7 +202,7 @@ static int kv_check(const char *what, const wt_kv_cache *c, int dtype, const int
         return WT_E_BADARG;
     }
     if (!table || n_seqs < 0 || table_width <= 0 || (n_seqs > 1 && table_stride < table_width) ||
-        (int64_t)table_width * c->page_size > 0x7fffffffll) {
+        (int64_t)table_width * c->page_size > WT_KV_MAX_POSITIONS) {
         set_error("%s: bad table (%d sequences of %d pages, %lld apart)", what, n_seqs, table_width, (long long)table_stride);
         return WT_E_BADARG;
     }
@@ -319,12 +319,17 @@ static int kv_plan(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_wi
     const int group = n_q_heads / c->n_heads;
     const int64_t pairs = (int64_t)n_seqs * c->n_heads * ((group + 15) / 16);
     const int64_t key_bytes = 2ll * c->head_dim * (c->dtype == WT_DTYPE_F32 ? 4 : c->dtype == WT_DTYPE_E4M3 ? 1 : 2);   // and its value's
-    p->n_wg = n < WT_KV_WORKSPACE_ZEROED / 4 ? n : WT_KV_WORKSPACE_ZEROED / 4;
+    p->n_wg = n < WT_KV_WORKSPACE_ZEROED / 16 ? n : WT_KV_WORKSPACE_ZEROED / 16;   // (four counters each)
     p->min_share = 4;
     p->seg_cost = 2;
+    // One workgroup streams 512 KB of keys and values in about the time that splitting them costs (measured, 8 to 640 pairs in
+    // four types: 256 KB 9.6 us against 13.3, 512 KB 13.9 against 14.7, 1 MB 27.6 against 16.2).  With as many pairs as keep
+    // every wave slot busy, a wave each is better still: 5120 pairs of 32 / 128 / 448 keys 15.6 / 33.7 / 94.7 us against 17.8 /
+    // 50.0 / 113; 768 pairs of 256 keys 13.1 against 13.4, of 448 19.7 against 19.3.
     p->direct = (int64_t)table_width * c->page_size * key_bytes <= 512 * 1024;
-    p->grid = p->direct ? (unsigned)pairs : (unsigned)p->n_wg;
-    p->bytes = p->direct ? 0 : WT_KV_WORKSPACE_ZEROED + (int64_t)p->n_wg * 2 * (32 + 16 * c->head_dim) * 4;
+    if (p->direct && pairs >= 8 * n) p->direct = 2;
+    p->grid = p->direct == 0 ? (unsigned)p->n_wg : p->direct == 1 ? (unsigned)pairs : (unsigned)((pairs + 3) / 4);
+    p->bytes = p->direct ? 0 : WT_KV_WORKSPACE_ZEROED + (int64_t)p->n_wg * 2 * kv_slot(c->head_dim) * 4;
     return WT_OK;
 }
 
@@ -378,7 +383,7 @@ int kv_attend(const wt_kv_cache *c, const void *q, int dtype, int64_t q_row, int
             WT_HIP(hipStreamIsCapturing(st, &cap));
             if (cap != hipStreamCaptureStatusNone) {
                 set_error("wt_kv_attend: a captured call needs a workspace of its own (%lld bytes)", (long long)p.bytes);
-                return WT_E_BADARG;
+                return WT_E_CAPTURE;
             }
             bool fresh = false;
             if ((rc = scratch_kv(st, (size_t)p.bytes, &workspace, &fresh))) return rc;
@@ -391,6 +396,7 @@ int kv_attend(const wt_kv_cache *c, const void *q, int dtype, int64_t q_row, int
     a.n_q_heads = n_q_heads, a.group = n_q_heads / c->n_heads, a.q_tiles = (a.group + 15) / 16;
     a.scale = scale, a.lengths = lengths, a.out = out, a.o_row = o_row, a.o_head = o_head, a.lse = lse;
     a.q_aligned = (((uintptr_t)q | (uint64_t)(q_row * item) | (uint64_t)(q_head * item)) & 15) == 0;
+    a.o_aligned = (((uintptr_t)out | (uint64_t)(o_row * item) | (uint64_t)(o_head * item)) & (4 * item - 1)) == 0;
     a.direct = p.direct, a.n_wg = p.n_wg, a.min_share = p.min_share, a.seg_cost = p.seg_cost;
     a.counters = (int32_t *)workspace;
     a.partials = workspace ? (float *)((char *)workspace + WT_KV_WORKSPACE_ZEROED) : nullptr;

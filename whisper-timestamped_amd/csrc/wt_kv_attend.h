@@ -17,7 +17,7 @@ constexpr float KV_LOG2E = 1.44269504088896340736f;
 // CT: what the pages hold; T: queries and results.
 // Matrix instructions take 16-bit operands as they are; 8-bit codes become bf16 (exactly), and then the queries are split
 // into bf16 parts whose sum they are: bf16 1, f16 2, f32 3.  f32 pages use the f32 instruction.
-template <typename CT, typename T>
+template <typename CT, typename T, int HD>
 struct KvKind {
     static constexpr bool F32 = sizeof(CT) == 4, E4M3 = sizeof(CT) == 1;
     static constexpr bool F16 = !F32 && !E4M3 && __is_same(CT, f16_t);
@@ -41,7 +41,7 @@ __device__ __forceinline__ constexpr int kv_d(int s, int g) {
 
 template <typename CT, typename T, int HD>
 struct KvFrag {
-    using K = KvKind<CT, T>;
+    using K = KvKind<CT, T, HD>;
     static constexpr int STEPS = HD / (K::F32 ? 16 : 32), EV = HD / 16;
     static constexpr int KD = K::E4M3 ? 2 : 4;                                       // dwords a step and tile
     static constexpr int VD = (EV * (int)sizeof(CT) + 3) / 4;                        // dwords of a key's values
@@ -76,8 +76,8 @@ __device__ __forceinline__ void kv_fetch(uint32_t *dst, const char *src) {
 }
 
 // Where a block's rows are, for this lane: byte offsets from the tensors' starts.
-//   PG 32: a page size that 32 divides: the block is in one page, the offsets the wave's
-//   PG  8: one that 8 divides (f32: 4): each group of keys is in one page
+//   PG 32: a page size that the block divides: the block is in one page, the offsets the wave's
+//   PG  8: one that a lane group's GK keys (8, f32 4) divide: each group is in one page
 //   PG  1: any other: each key by itself
 template <int PG, int NT, int GK>
 struct KvSpot {
@@ -87,7 +87,7 @@ struct KvSpot {
 
 template <typename CT, typename T, int HD, int PG, int NW>
 struct KvWave {
-    using K = KvKind<CT, T>;
+    using K = KvKind<CT, T, HD>;
     using Frag = KvFrag<CT, T, HD>;
     using Spot = KvSpot<PG, K::NT, K::GK>;
     static constexpr int STEPS = Frag::STEPS, EV = Frag::EV, ITEM = sizeof(CT);
@@ -114,23 +114,23 @@ struct KvWave {
     __device__ __forceinline__ int kkey(int t) const { return (n >> 2) * K::GK + t * 4 + (n & 3); }
     __device__ __forceinline__ Ids ids(int p0) const { return ids(p0, len); }
     __device__ __forceinline__ Ids ids(int p0, int len) const {
+        Ids id;
         if constexpr (PG == 32) {
-            const int i = row[__builtin_amdgcn_readfirstlane((int)page_of(a.c.div, (uint32_t)min(p0, len - 1)))];
-            return {i, i};
+            id.k = id.v = row[__builtin_amdgcn_readfirstlane((int)page_of(a.c.div, (uint32_t)min(p0, len - 1)))];
         } else if constexpr (PG == 8) {
-            const int last = len - 1;
-            return {row[page_of(a.c.div, (uint32_t)min(p0 + (n >> 2) * K::GK, last))], row[page_of(a.c.div, (uint32_t)min(p0 + g * K::GK, last))]};
+            id.k = row[page_of(a.c.div, (uint32_t)min(p0 + (n >> 2) * K::GK, len - 1))];
+            id.v = row[page_of(a.c.div, (uint32_t)min(p0 + g * K::GK, len - 1))];
         } else {
-            const int i = row[page_of(a.c.div, (uint32_t)min(p0 + (lane & (K::KB - 1)), len - 1))];
-            return {i, i};
+            id.k = id.v = row[page_of(a.c.div, (uint32_t)min(p0 + (lane & (K::KB - 1)), len - 1))];
         }
+        return id;
     }
     __device__ __forceinline__ int checked(int page, bool *wrong) const {
         const bool w = (uint32_t)page >= (uint32_t)a.c.n_pages;
         *wrong |= w;
         return w ? 0 : page;
     }
-    __device__ __forceinline__ void place(int p0, Ids id, Spot &s) {
+    __device__ __forceinline__ void place(int p0, const Ids &id, Spot &s) {
         if constexpr (PG == 32) {
             const int page = checked(__builtin_amdgcn_readfirstlane(id.k), &bad);
             const int slot = p0 - (int)(page_of(a.c.div, (uint32_t)p0) * a.c.div.d);
@@ -138,7 +138,8 @@ struct KvWave {
             s.v[0] = (page * a.v.page + h * a.v.head + slot * a.v.slot) * ITEM;
             s.e[0] = ((int64_t)page * a.c.n_heads + h) * a.c.page_size + slot;
         } else if constexpr (PG == 8) {
-            const int pk = min(p0 + (n >> 2) * K::GK, (len - 1) & -K::GK), pv = min(p0 + g * K::GK, (len - 1) & -K::GK);
+            const int last = (len - 1) & -K::GK;
+            const int pk = min(p0 + (n >> 2) * K::GK, last), pv = min(p0 + g * K::GK, last);
             const int page_k = checked(id.k, &bad), page_v = checked(id.v, &bad);
             const int slot_k = pk - (int)(page_of(a.c.div, (uint32_t)pk) * a.c.div.d) + (n & 3);
             const int slot_v = pv - (int)(page_of(a.c.div, (uint32_t)pv) * a.c.div.d);
@@ -199,7 +200,10 @@ struct KvWave {
             if constexpr (PG == 1) {
                 uint32_t w[2][2] = {{0, 0}, {0, 0}};
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[0][j / 4] |= (uint32_t)a.k.e[s.e[j]] << (j % 4 * 8), w[1][j / 4] |= (uint32_t)a.v.e[s.e[j]] << (j % 4 * 8);
+                for (int j = 0; j < 8; ++j) {
+                    w[0][j / 4] |= (uint32_t)a.k.e[s.e[j]] << (j % 4 * 8);
+                    w[1][j / 4] |= (uint32_t)a.v.e[s.e[j]] << (j % 4 * 8);
+                }
                 f.ke = {w[0][0], w[0][1]}, f.ve = {w[1][0], w[1][1]};
             } else {
                 const int64_t e = s.e[0] + (PG == 32 ? g * 8 : 0);
@@ -305,14 +309,14 @@ struct KvWave {
         } else {
             // a weight is the sum of two 16-bit numbers: with one alone the result is off by up to 2^-9 (bf16) where few keys
             // share the weight; with both by less than 2^-16
+            // values arrive as rows (key j: EV neighbouring columns a lane) and are needed as columns: pairs of rows are
+            // interleaved by byte permutes
             u4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 hi[i] = pack16(p[2 * i], p[2 * i + 1]);
                 lo[i] = pack16(p[2 * i] - low16(hi[i]), p[2 * i + 1] - high16(hi[i]));
             }
-            // values arrive as rows (key j: EV neighbouring columns a lane) and are needed as columns: pairs of rows are
-            // interleaved by byte permutes
             uint32_t w[8][EV / 2];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -427,9 +431,29 @@ __device__ __forceinline__ uint32_t kv_div(uint64_t x, uint64_t y) {   // where 
 }
 
 // Partial results travel between workgroups, which may run on different XCDs with an L2 each: stored through to memory and
-// loaded from there.  (Fences of the agent's scope around plain stores write back and invalidate whole L2s.)
-__device__ __forceinline__ void kv_put(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float kv_get(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// loaded from there (the agent's scope in the instruction itself).  Fences of that scope around plain stores write back and
+// invalidate whole L2s: with them, 131071 positions took 246 us instead of 171.
+constexpr int KV_AGENT = 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t kv_partials(const KvAttend &a) {
+    return __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, a.n_wg * 2 * kv_slot(a.c.head_dim) * 4, 0x00020000);
+}
+__device__ __forceinline__ void kv_put(__amdgpu_buffer_rsrc_t p, int at, float v) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), p, at * 4, 0, KV_AGENT); }
+__device__ __forceinline__ void kv_put(__amdgpu_buffer_rsrc_t p, int at, f4 v) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), p, at * 4, 0, KV_AGENT); }
+__device__ __forceinline__ float kv_get(__amdgpu_buffer_rsrc_t p, int at) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(p, at * 4, 0, KV_AGENT)); }
+__device__ __forceinline__ f4 kv_get4(__amdgpu_buffer_rsrc_t p, int at) { return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(p, at * 4, 0, KV_AGENT)); }
+
+template <typename T>
+__device__ __forceinline__ void kv_result(const KvAttend &a, int s, int head, int d, f4 v) {
+    T *dst = static_cast<T *>(a.out) + s * a.o_row + head * a.o_head + d;
+    Pack<T, 4> out;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) out.v[x] = from_f<T>(v[x]);
+    if (a.o_aligned) *reinterpret_cast<Pack<T, 4> *>(dst) = out;
+    else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) dst[x] = out.v[x];
+    }
+}
 
 // One workgroup's part of one (sequence, key head, query tile): blocks [b0, b1).  What the waves found is joined in LDS and
 // goes out as the result, or as a partial one (slot >= 0).  LATE: the length is not known yet (all blocks are meant then):
@@ -437,7 +461,7 @@ __device__ __forceinline__ float kv_get(const float *p) { return __hip_atomic_lo
 template <bool LATE, typename CT, typename T, int HD, int PG, int NW>
 __device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW> &w, const KvAttend &a, float *lds, int s, int pair, int len, bool bad_len,
                                            int b0, int b1, int slot) {
-    constexpr int EV = HD / 16, KB = KvKind<CT, T>::KB;
+    constexpr int EV = HD / 16, KB = KvKind<CT, T, HD>::KB;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = pair / a.q_tiles, qt = pair % a.q_tiles;
     const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
     w.row = a.t.t + s * a.t.stride;
@@ -467,69 +491,66 @@ __device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW> &w, const K
             for (int i = 0; i < EV; ++i) lo[(wave * rows + w.n) * HD + (4 * w.g + r) * EV + i] = w.o[i][r];
     }
     __syncthreads();
-    float *part = slot >= 0 ? a.partials + (int64_t)slot * (32 + 16 * HD) : nullptr;
-    for (int e = threadIdx.x; e < rows * HD; e += NW * 64) {
-        const int r = e / HD, d = e % HD;
+    const __amdgpu_buffer_rsrc_t part = kv_partials(a);
+    const int at = slot * kv_slot(HD);
+    for (int e = threadIdx.x; e < rows * (HD / 4); e += NW * 64) {
+        const int r = e / (HD / 4), d = e % (HD / 4) * 4;
         float mm = lm[r];
 #pragma unroll
         for (int i = 1; i < NW; ++i) mm = fmaxf(mm, lm[i * 16 + r]);
-        float acc = 0.f, sum = 0.f;
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const float c = __builtin_amdgcn_exp2f((lm[i * 16 + r] - mm) * KV_LOG2E);
-            acc = fmaf(lo[(i * rows + r) * HD + d], c, acc);
+            const f4 x = *reinterpret_cast<const f4 *>(&lo[(i * rows + r) * HD + d]);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) acc[y] = fmaf(x[y], c, acc[y]);
             sum = fmaf(ll[i * 16 + r], c, sum);
         }
-        if (part) {
-            kv_put(part + 32 + e, acc);
-            if (d == 0) kv_put(part + r, mm), kv_put(part + 16 + r, sum);
+        if (slot >= 0) {
+            kv_put(part, at + 64 + e * 4, acc);
+            if (d == 0) kv_put(part, at + r, mm), kv_put(part, at + 16 + r, sum);
         } else {
             const bool empty = len == 0 && !bad_len;
-            static_cast<T *>(a.out)[s * a.o_row + (hq0 + r) * a.o_head + d] = from_f<T>(empty ? 0.f : acc / sum);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) acc[y] = empty ? 0.f : acc[y] / sum;
+            kv_result<T>(a, s, hq0 + r, d, acc);
             if (a.lse && d == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + r] = empty ? -__builtin_inff() : mm + logf(sum);
         }
     }
 }
 
 // The last workgroup of a pair to arrive joins its partial results.  A thread takes four columns of a row, and where there
-// are more threads than that, every LANES-th part; JOIN parts are loaded at a time, in an order that never changes.
-constexpr int KV_JOIN = 8;
-template <typename T, int HD, int NW>
-__device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, int pair, int first_wg, int n_parts) {
-    wait_vmcnt0();     // every wave's stores are where the others read them before the count
-    __syncthreads();   // (and lds is free)
-    int *last = reinterpret_cast<int *>(lds);
-    if (threadIdx.x == 0) {
-        const int before = atomicAdd(&a.counters[first_wg], 1);
-        *last = before == n_parts - 1;
-        if (before == n_parts - 1) a.counters[first_wg] = 0;
-    }
-    __syncthreads();
-    if (!*last) return;
-    __syncthreads();   // (lds is free again)
-    const int h = pair / a.q_tiles, qt = pair % a.q_tiles;
-    const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
-    constexpr int64_t SLOT = 32 + 16 * HD;
+// are more threads than that, every LANES-th part; KV_JOIN parts are loaded at a time, in an order that never changes.  With
+// more than two KV_GROUPs of parts the last of each group joins the group, and the last of those the groups (90 parts of 8
+// queries of 256 values: 30 us by one workgroup alone).
+constexpr int KV_JOIN = 8, KV_GROUP = 16;
+
+// parts first, first + step, ... (count of them; number i stands in slot_of(i), its maxima and sums `stats` floats into it) ->
+// the result, or one part, in the slot of `first`, its maxima and sums in the second place for them
+template <typename T, int HD, int NW, typename SlotOf>
+__device__ __forceinline__ void kv_reduce(const KvAttend &a, float *lds, int s, int hq0, int rows, SlotOf slot_of, int first, int step, int count,
+                                          int stats, bool result) {
     constexpr int NTH = NW * 64;
+    const __amdgpu_buffer_rsrc_t parts = kv_partials(a);
     const int quads = rows * (HD / 4);
-    const int lanes = min(max(NTH / quads, 1), n_parts);   // threads that share four columns
-    // the first part stands in the slot of a segment that goes on, the others in that of one that came from before
-    const auto part = [&](int i) { return a.partials + (i == 0 ? 2 * (int64_t)first_wg + 1 : 2 * (int64_t)(first_wg + i)) * SLOT; };
+    const int lanes = min(max(NTH / quads, 1), count);   // threads that share four columns
     for (int e0 = 0; e0 < quads; e0 += NTH / lanes) {
         const int e = e0 + threadIdx.x / lanes, mine = threadIdx.x % lanes;
         const bool in = e < quads && threadIdx.x / lanes < NTH / lanes;
         const int r = in ? e / (HD / 4) : 0, d = in ? e % (HD / 4) * 4 : 0;
         float mm = KV_LOWEST, sum = 0.f;
         f4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int i0 = mine; i0 < n_parts; i0 += lanes * KV_JOIN) {
-            float m[KV_JOIN], l[KV_JOIN], o[KV_JOIN][4];
+        for (int i0 = mine; i0 < count; i0 += lanes * KV_JOIN) {
+            float m[KV_JOIN], l[KV_JOIN];
+            f4 o[KV_JOIN];
 #pragma unroll
             for (int i = 0; i < KV_JOIN; ++i) {
-                const bool there = i0 + i * lanes < n_parts;
-                const float *p = part(there ? i0 + i * lanes : i0);
-                m[i] = kv_get(p + r), l[i] = kv_get(p + 16 + r);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[i][x] = kv_get(p + 32 + r * HD + d + x);
+                const bool there = i0 + i * lanes < count;
+                const int p = slot_of(first + (there ? i0 + i * lanes : i0) * step) * kv_slot(HD);
+                m[i] = kv_get(parts, p + stats + r), l[i] = kv_get(parts, p + stats + 16 + r);
+                o[i] = kv_get4(parts, p + 64 + r * HD + d);
             }
             float mn = mm;
 #pragma unroll
@@ -538,7 +559,7 @@ __device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, in
             sum *= c, acc *= c, mm = mn;
 #pragma unroll
             for (int i = 0; i < KV_JOIN; ++i) {
-                const bool there = i0 + i * lanes < n_parts;
+                const bool there = i0 + i * lanes < count;
                 const float w = __builtin_amdgcn_exp2f((m[i] - mm) * KV_LOG2E);
                 if (there) {
                     sum = fmaf(l[i], w, sum);
@@ -566,25 +587,119 @@ __device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, in
             __syncthreads();
         }
         if (in && mine == 0) {
-            T *dst = static_cast<T *>(a.out) + s * a.o_row + (hq0 + r) * a.o_head + d;
+            if (result) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) dst[x] = from_f<T>(acc[x] / sum);
-            if (a.lse && d == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + r] = mm + logf(sum);
+                for (int x = 0; x < 4; ++x) acc[x] /= sum;
+                kv_result<T>(a, s, hq0 + r, d, acc);
+                if (a.lse && d == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + r] = mm + logf(sum);
+            } else {   // (only this thread reads these columns of the slot; its maxima others may still read)
+                const int p = slot_of(first) * kv_slot(HD);
+                kv_put(parts, p + 64 + r * HD + d, acc);
+                if (d == 0) kv_put(parts, p + 32 + r, mm), kv_put(parts, p + 48 + r, sum);
+            }
         }
+    }
+}
+
+// Counts this workgroup's arrival, its stores being out; true in the last of `of`, which leaves the counter at zero.
+__device__ __forceinline__ bool kv_last(int32_t *counter, int of, float *lds) {
+    wait_vmcnt0();     // every wave's stores are where the others read them before the count
+    __syncthreads();   // (and lds is free)
+    int *last = reinterpret_cast<int *>(lds);
+    if (threadIdx.x == 0) {
+        const int before = atomicAdd(counter, 1);
+        *last = before == of - 1;
+        if (before == of - 1) *counter = 0;
+    }
+    __syncthreads();
+    const bool is = *last;
+    __syncthreads();   // (lds is free again)
+    return is;
+}
+
+template <typename T, int HD, int NW>
+__device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, int pair, int first_wg, int n_parts) {
+    const int h = pair / a.q_tiles, qt = pair % a.q_tiles;
+    const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
+    // the first part stands in the slot of a segment that goes on, the others in that of one that came from before
+    const auto slot_of = [&](int i) { return 2 * (first_wg + i) + (i == 0 ? 1 : 0); };
+    const bool grouped = n_parts > 2 * KV_GROUP;
+    int first = grouped ? (int)(blockIdx.x - first_wg) / KV_GROUP * KV_GROUP : 0;
+    int count = grouped ? min(KV_GROUP, n_parts - first) : n_parts, step = 1;
+    int32_t *counter = a.counters + slot_of(first);
+    while (kv_last(counter, count, lds)) {
+        const bool result = !grouped || step > 1;
+        kv_reduce<T, HD, NW>(a, lds, s, hq0, rows, slot_of, first, step, count, step > 1 ? 32 : 0, result);
+        if (result) return;
+        first = 0, step = KV_GROUP, count = (n_parts + KV_GROUP - 1) / KV_GROUP;
+        counter = a.counters + 2 * a.n_wg + slot_of(0);
+    }
+}
+
+// Short tables: one workgroup of NW waves per (sequence, key head, query tile); one wave, four pairs a workgroup, where a
+// pair's keys are few or the pairs many.
+template <typename CT, typename T, int HD, int PG, int NW>
+__global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_direct_kernel(const KvAttend a) {
+    extern __shared__ __attribute__((aligned(16))) float kv_lds[];
+    const unsigned pairs = a.c.n_heads * a.q_tiles;
+    KvWave<CT, T, HD, PG, NW> w(a);
+    kv_segment<true, CT, T, HD, PG, NW>(w, a, kv_lds, blockIdx.x / pairs, blockIdx.x % pairs, 0, false, 0, 0, -1);
+}
+
+template <typename CT, typename T, int HD, int PG>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void kv_attend_wave_kernel(const KvAttend a) {
+    constexpr int EV = HD / 16, KB = KvKind<CT, T, HD>::KB;
+    const unsigned pairs = a.c.n_heads * a.q_tiles;
+    const unsigned at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int s = at / pairs, pair = at % pairs;
+    if (s >= a.t.n_seqs) return;
+    const int h = pair / a.q_tiles, qt = pair % a.q_tiles;
+    const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
+    KvWave<CT, T, HD, PG, 1> w(a);
+    w.row = a.t.t + s * a.t.stride;
+    w.h = h;
+    typename KvWave<CT, T, HD, PG, 1>::Raw raw;
+    const int raw_len = a.lengths[s];
+    const auto first = w.ids(0, (int)kv_capacity(a));
+    w.queries_load(raw, s, hq0, rows);
+    bool bad_len;
+    const int len = __builtin_amdgcn_readfirstlane(kv_length(a, raw_len, &bad_len));
+    w.len = len;
+    w.bad = bad_len;
+    w.run(0, (len + KB - 1) / KB, first, raw, rows);
+    const bool bad = __any(w.bad);
+    if (bad && w.lane == 0) kv_report(a.c.error, bad_len ? WT_KV_BAD_POSITION : WT_KV_BAD_PAGE);
+    float l = w.l;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (bad) l = __builtin_nanf("");
+    const bool empty = len == 0 && !bad_len;
+    if (w.n < rows) {
+        constexpr int C = EV % 4 == 0 ? 4 : 2;
+        const float inv = empty ? 0.f : 1.f / l;
+        T *dst = static_cast<T *>(a.out) + s * a.o_row + (hq0 + w.n) * a.o_head + w.g * 4 * EV;
+#pragma unroll
+        for (int e = 0; e < 4 * EV; e += C) {
+            Pack<T, C> v;
+#pragma unroll
+            for (int x = 0; x < C; ++x) v.v[x] = from_f<T>(empty ? 0.f : w.o[(e + x) % EV][(e + x) / EV] * inv);
+            if (a.o_aligned) *reinterpret_cast<Pack<T, C> *>(dst + e) = v;
+            else {
+#pragma unroll
+                for (int x = 0; x < C; ++x) dst[e + x] = v.v[x];
+            }
+        }
+        if (a.lse && w.g == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + w.n] = empty ? -__builtin_inff() : w.m + logf(l);
     }
 }
 
 template <typename CT, typename T, int HD, int PG, int NW>
 __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_kernel(const KvAttend a) {
     extern __shared__ __attribute__((aligned(16))) float kv_lds[];
-    constexpr int KB = KvKind<CT, T>::KB, UNIT = KB * NW;
+    constexpr int KB = KvKind<CT, T, HD>::KB, UNIT = KB * NW;
     const int lane = threadIdx.x & 63;
     const int pairs = a.c.n_heads * a.q_tiles;   // of one sequence
     KvWave<CT, T, HD, PG, NW> w(a);
-    if (a.direct) {
-        kv_segment<true, CT, T, HD, PG, NW>(w, a, kv_lds, blockIdx.x / pairs, blockIdx.x % pairs, 0, false, 0, 0, -1);
-        return;
-    }
     // All pairs stand in a row, sequence by sequence, each with seg_cost units for what a segment costs by itself (queries,
     // joining the waves) and then one for every NW blocks of keys; workgroup i takes the i-th share of the row.
     const int n_seqs = a.t.n_seqs, head = a.seg_cost;
@@ -660,21 +775,23 @@ static int kv_attend_go(const KvAttend &a, unsigned grid, hipStream_t st) {
     const int rows = a.group < 16 ? a.group : 16;
     size_t lds = sizeof(float) * NW * (32 + (size_t)rows * HD);
     if (lds < sizeof(float) * NW * 64 * 6) lds = sizeof(float) * NW * 64 * 6;   // what the join of partial results takes
-    if (lds > 64 * 1024) {
-        static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void *>(kv_attend_kernel<CT, T, HD, PG, NW>),
-                                                           hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-        WT_HIP(once);
-    }
-    hipLaunchKernelGGL((kv_attend_kernel<CT, T, HD, PG, NW>), dim3(grid), dim3(NW * 64), lds, st, a);
+    const auto kernel = a.direct == 0   ? kv_attend_kernel<CT, T, HD, PG, NW>
+                        : a.direct == 1 ? kv_attend_direct_kernel<CT, T, HD, PG, NW>
+                                        : kv_attend_wave_kernel<CT, T, HD, PG>;
+    if (a.direct == 2) lds = 0;
+    if (lds > 64 * 1024)   // (16 queries of 256 values)
+        WT_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, st, a);
     WT_HIP(hipGetLastError());
     return WT_OK;
 }
+
 // page sizes: see KvSpot
 template <typename CT, typename T, int HD>
 static int kv_attend_pages(const KvAttend &a, unsigned grid, hipStream_t st) {
-    constexpr int GK = KvKind<CT, T>::GK;
-    if (a.c.page_size % 32 == 0) return kv_attend_go<CT, T, HD, 32>(a, grid, st);
-    if (a.c.page_size % GK == 0) return kv_attend_go<CT, T, HD, 8>(a, grid, st);
+    using K = KvKind<CT, T, HD>;
+    if (a.c.page_size % K::KB == 0) return kv_attend_go<CT, T, HD, 32>(a, grid, st);
+    if (a.c.page_size % K::GK == 0) return kv_attend_go<CT, T, HD, 8>(a, grid, st);
     return kv_attend_go<CT, T, HD, 1>(a, grid, st);
 }
 

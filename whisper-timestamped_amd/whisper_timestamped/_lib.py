@@ -36,7 +36,8 @@ EXPORTS = ["wt_version", "wt_last_error", "wt_shutdown", "wt_cost_batch", "wt_dt
 WT_STEP_SYMMETRIC1, WT_STEP_NO_EMPTY_SUBWORDS = 0, 1
 ABI_VERSION = 5
 WT_KV_BAD_POSITION, WT_KV_BAD_PAGE, WT_KV_BAD_SEQUENCE = 1, 2, 4
-WT_KV_WORKSPACE_ZEROED = 16384
+WT_KV_WORKSPACE_ZEROED, WT_KV_MAX_POSITIONS = 16384, 0x7fffff00
+WT_E_CAPTURE = -4
 WT_ALIGN_KEEP_COST, WT_ALIGN_NO_FUSED_SMALL_UNITS, WT_ALIGN_ROWS_PER_CLASS = 1, 2, 4
 
 

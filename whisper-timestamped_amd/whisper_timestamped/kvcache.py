@@ -118,20 +118,20 @@ class PagedKVCache:
         return dt
 
     def _int32(self, t, name, n):
-        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != self.device or t.dim() != 1 or t.shape[0] != n or \
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != self._index or t.shape != (n,) or \
                 not t.is_contiguous():
             raise WtError(f"{name}: {n} contiguous int32 on {self.device}")
         return t.data_ptr()
 
     def _table(self, table):
-        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype is not torch.int32 or table.device != self.device:
+        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != self._index:
             raise WtError(f"page table: int32 (sequences, pages) on {self.device}")
         n, width = table.shape
         stride, one = table.stride()
         if width < 1 or (one != 1 and width > 1) or (n > 1 and stride < width):
             raise WtError("page table: the pages of a sequence stand side by side, its rows apart")
-        if width * self.page_size > 2 ** 31 - 1:
-            raise WtError(f"page table: {width} pages of {self.page_size} are beyond 32-bit positions")
+        if width * self.page_size > _lib.WT_KV_MAX_POSITIONS:
+            raise WtError(f"page table: {width} pages of {self.page_size} are more than {_lib.WT_KV_MAX_POSITIONS} positions")
         return table.data_ptr(), stride if n > 1 else width, n, width
 
     def _rows_of(self, positions, sequences, n_seqs):
@@ -144,7 +144,7 @@ class PagedKVCache:
         return n, None if sequences is None else self._int32(sequences, "sequences", n), pos
 
     def _new(self, t, name, n):
-        if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.device != self.device or tuple(t.shape) != (n, self.n_heads, self.head_dim):
+        if not isinstance(t, torch.Tensor) or t.get_device() != self._index or t.shape != (n, self.n_heads, self.head_dim):
             raise WtError(f"{name}: ({n}, {self.n_heads}, {self.head_dim}) on {self.device}")
         row, head, one = t.stride()
         row, head = row if n > 1 else 0, head if self.n_heads > 1 else 0
@@ -153,15 +153,12 @@ class PagedKVCache:
             raise WtError(f"{name}: rows must be contiguous and start on 16-byte steps (strides {t.stride()})")
         return p, row, head
 
-    def _call(self, entry, what, *args):
-        """The entry on the current stream of the cache's device."""
+    def _call(self, entry, *args):
+        """The entry on the current stream of the cache's device -> its return code."""
         if _current_device() == self._index:
-            rc = entry(self._p, *args, _raw_stream(self._index))
-        else:
-            with torch.cuda.device(self.device):
-                rc = entry(self._p, *args, _raw_stream(self._index))
-        if rc:
-            _lib._check(rc, what)
+            return entry(self._p, *args, _raw_stream(self._index))
+        with torch.cuda.device(self.device):
+            return entry(self._p, *args, _raw_stream(self._index))
 
     # --- operators
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, sequences: torch.Tensor | None = None):
@@ -176,7 +173,9 @@ class PagedKVCache:
             raise WtError(f"k and v differ: {k.dtype}, {v.dtype}")
         dt = self._dtype(k.dtype, "k, v")
         if n:
-            self._call(self._append, "wt_kv_append", kp, vp, dt, k_row, k_head, v_row, v_head, n, tp, ts, n_seqs, width, seq, pos)
+            rc = self._call(self._append, kp, vp, dt, k_row, k_head, v_row, v_head, n, tp, ts, n_seqs, width, seq, pos)
+            if rc:
+                _lib._check(rc, "wt_kv_append")
 
     def gather(self, table: torch.Tensor, positions: torch.Tensor, sequences: torch.Tensor | None = None, dtype=None, out=None):
         """-> (k, v), each (rows, heads, head_dim): the rows at ``positions[r]`` of sequence ``sequences[r]``, in the cache's
@@ -202,7 +201,9 @@ class PagedKVCache:
             if n and k.data_ptr() == v.data_ptr():
                 raise WtError("out: the same memory twice")
         if n:
-            self._call(self._gather, "wt_kv_gather", k.data_ptr(), v.data_ptr(), dt, n, tp, ts, n_seqs, width, seq, pos)
+            rc = self._call(self._gather, k.data_ptr(), v.data_ptr(), dt, n, tp, ts, n_seqs, width, seq, pos)
+            if rc:
+                _lib._check(rc, "wt_kv_gather")
         return out
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, scale: float | None = None,
@@ -217,7 +218,7 @@ class PagedKVCache:
         captured into a graph has none of the stream's: without ``workspace`` it takes one in the graph's memory, which
         costs every replay a small kernel that clears its counters."""
         tp, ts, n_seqs, width = self._table(table)
-        if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.device != self.device:
+        if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.get_device() != self._index:
             raise WtError(f"q: (sequences, query heads, head_dim) on {self.device}")
         n, hq, d = q.shape
         q_row, q_head, one = q.stride()
@@ -237,15 +238,17 @@ class PagedKVCache:
         if n:
             wp, w_bytes = None, 0
             if workspace is not None:
-                if workspace.dtype is not torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
+                if workspace.dtype is not torch.uint8 or workspace.get_device() != self._index or not workspace.is_contiguous():
                     raise WtError("workspace: what attend_workspace() gave")
                 wp, w_bytes = workspace.data_ptr(), workspace.numel()
-            elif torch.cuda.is_current_stream_capturing():
+            args = (self._attend, q.data_ptr(), dt, q_row, q_head, n, hq, self._scale if scale is None else scale, tp, ts, width, lp,
+                    out.data_ptr(), o_row, o_head, lse.data_ptr() if return_lse else None)
+            rc = self._call(*args, wp, w_bytes)
+            if rc == _lib.WT_E_CAPTURE and workspace is None:
                 workspace = self.attend_workspace(hq, table)
-                if workspace is not None:
-                    wp, w_bytes = workspace.data_ptr(), workspace.numel()
-            self._call(self._attend, "wt_kv_attend", q.data_ptr(), dt, q_row, q_head, n, hq, self._scale if scale is None else scale, tp, ts,
-                       width, lp, out.data_ptr(), o_row, o_head, lse.data_ptr() if return_lse else None, wp, w_bytes)
+                rc = self._call(*args, workspace.data_ptr(), workspace.numel())
+            if rc:
+                _lib._check(rc, "wt_kv_attend")
         return (out, lse) if return_lse else out
 
     def attend_workspace(self, n_q_heads: int, table: torch.Tensor) -> torch.Tensor | None:
