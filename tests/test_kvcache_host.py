@@ -110,3 +110,111 @@ def test_cache_descriptor_matches_the_header():
     assert ctypes.sizeof(_lib.KvCache) == 112
     assert [getattr(_lib.KvCache, n).offset for n in ("k", "v_exp", "k_page_stride", "v_slot_stride", "n_pages", "head_dim", "dtype", "error")] == \
         [0, 24, 32, 72, 80, 92, 96, 104]
+
+
+# The calls' own checks, on a cache whose tensors are the host's: what is right but for that is refused at the end.
+def host_cache(dtype=torch.float16, heads=2, page=16, width=64):
+    from whisper_timestamped import kvcache
+    cache = object.__new__(PagedKVCache)
+    cache.k, cache.v = pages(4, heads, page, width, dtype=dtype), pages(4, heads, page, width, dtype=dtype)
+    e = pages(4, heads, page, dtype=torch.uint8).data_ptr() if dtype == E4M3 else None
+    cache._keep = desc(k=cache.k.data_ptr(), v=cache.v.data_ptr(), k_exp=e, v_exp=e, n_heads=heads, page_size=page, head_dim=width,
+                       dtype=kvcache._PAGE_DTYPES[dtype])
+    cache._calls = kvcache._calls()
+    cache._handle = cache._calls.handle(ctypes.addressof(cache._keep), cache.k)
+    return cache
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+TABLE = torch.zeros((3, 4), dtype=torch.int32)
+ROWS = pages(3, 2, 64)
+
+
+@pytest.mark.parametrize("change,said", [
+    ({}, "only run on the GPU"),
+    (dict(k=None), "k: not a tensor"),
+    (dict(k=pages(3, 2, 64, dtype=torch.float32)), "k and v differ"),
+    (dict(k=pages(3, 2, 64, dtype=torch.float32), v=pages(3, 2, 64, dtype=torch.float32)), "Float with a cache of Half"),
+    (dict(v=pages(3, 1, 64)), r"v: \(3, 1, 64\), not \(3, 2, 64\)"),
+    (dict(k=pages(3, 128)), "k: 2 dimensions"),
+    (dict(k=pages(3, 2, 128)[..., ::2]), "k: a head's values stand side by side"),
+    (dict(k=pages(3, 2, 65)[..., :64]), "16-byte"),
+    (dict(k=pages(3, 2, 72)[..., 4:68]), "16-byte"),
+    (dict(positions=i32(0, 1)), r"k: \(3, 2, 64\), not \(2, 2, 64\)"),
+    (dict(positions=torch.zeros(3)), "positions: 3 int32"),
+    (dict(positions=torch.zeros(3, dtype=torch.int64)), "positions: 3 int32"),
+    (dict(positions=torch.zeros((3, 1), dtype=torch.int32)), "positions: 2 dimensions"),
+    (dict(positions=torch.zeros(6, dtype=torch.int32)[::2]), "side by side"),
+    (dict(sequences=i32(0, 1)), "sequences: 3 int32"),
+    (dict(k=pages(4, 2, 64), v=pages(4, 2, 64), positions=i32(0, 1, 2, 3)), "4 rows for 3 sequences"),
+    (dict(table=TABLE.long()), "page table: not int32"),
+    (dict(table=TABLE[0]), "page table: 1 dimensions"),
+    (dict(table=TABLE.t().contiguous().t()), "side by side"),
+    (dict(table=TABLE[:1].expand(3, 4)), "its rows apart"),
+    (dict(table=torch.zeros((3, 0), dtype=torch.int32)), "page table"),
+])
+def test_append_arguments(change, said):
+    a = dict(k=ROWS, v=ROWS, table=TABLE, positions=i32(0, 1, 2), sequences=None)
+    with pytest.raises(WtError, match=said):
+        host_cache().append(**dict(a, **change))
+
+
+@pytest.mark.parametrize("dtype,change,said", [
+    (torch.float16, {}, "only run on the GPU"),
+    (torch.float16, dict(dtype=torch.float32), "Float with a cache of Half"),
+    (E4M3, dict(dtype=torch.float64), "Double"),
+    (E4M3, dict(dtype=E4M3), "Float8"),
+    (E4M3, dict(dtype=torch.bfloat16), "only run on the GPU"),
+    (torch.float16, dict(dtype="float16"), "torch.dtype"),
+    (torch.float16, dict(out=ROWS), "out: two tensors"),
+    (torch.float16, dict(out=(ROWS, ROWS)), "the same memory"),
+    (torch.float16, dict(out=(ROWS, pages(2, 2, 64))), r"out\[1\]"),
+    (torch.float16, dict(out=(ROWS, pages(3, 2, 64, dtype=torch.float32))), "out: Half and Float"),
+    (torch.float16, dict(out=(pages(3, 4, 64)[:, :2], ROWS)), "not contiguous"),
+    (torch.float16, dict(out=(ROWS, pages(3, 2, 64)), dtype=torch.bfloat16), "out: Half"),
+    (torch.float16, dict(positions=torch.zeros(3)), "positions"),
+])
+def test_gather_arguments(dtype, change, said):
+    a = dict(table=TABLE, positions=i32(0, 1, 2), sequences=None, dtype=None, out=None)
+    with pytest.raises(WtError, match=said):
+        host_cache(dtype).gather(**dict(a, **change))
+
+
+Q = pages(3, 4, 64)
+
+
+@pytest.mark.parametrize("change,said", [
+    ({}, "only run on the GPU"),
+    (dict(q=pages(3, 3, 64)), "3 query heads over 2"),
+    (dict(q=pages(3, 0, 64)), "0 query heads"),
+    (dict(q=pages(2, 4, 64)), r"q: \(2, 4, 64\), not \(3, 4, 64\)"),
+    (dict(q=pages(3, 4, 32)), "q:"),
+    (dict(q=pages(3, 4, 64, dtype=torch.bfloat16)), "BFloat16 with a cache of Half"),
+    (dict(q=pages(3, 4, 128)[..., ::2]), "side by side"),
+    (dict(lengths=torch.zeros(3)), "lengths"),
+    (dict(lengths=i32(1, 2)), "lengths: 3 int32"),
+    (dict(out=pages(3, 4, 64, dtype=torch.float32)), "out: Float"),
+    (dict(out=3), "out: not a tensor"),
+    (dict(out=pages(1, 4, 64).expand(3, 4, 64)), "one place"),
+    (dict(out=pages(3, 1, 64).expand(3, 4, 64)), "one place"),
+    (dict(out=torch.zeros(3 * 64 + 512, dtype=torch.float16).as_strided((3, 4, 64), (64, 64, 1))), "one place"),
+    (dict(out=torch.zeros(12 * 64, dtype=torch.float16).as_strided((3, 4, 64), (64, 192, 1))), "only run on the GPU"),
+    (dict(workspace=pages(100)), "workspace"),
+    (dict(table=TABLE[:2]), "q:"),
+])
+def test_attend_arguments(change, said):
+    a = dict(q=Q, table=TABLE, lengths=i32(1, 2, 3))
+    with pytest.raises(WtError, match=said):
+        host_cache().attend(**dict(a, **change))
+
+
+def test_attend_wrong_python_types():
+    with pytest.raises(TypeError):
+        host_cache().attend(Q, TABLE, i32(1, 2, 3), scale="x")
+    with pytest.raises(TypeError):
+        host_cache().attend_workspace("x", TABLE)
+    with pytest.raises(WtError, match="0 query heads"):
+        host_cache().attend_workspace(0, TABLE)

@@ -19,6 +19,7 @@ and returns NaN for what it could not compute.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -28,14 +29,19 @@ from ._lib import WtError
 _DTYPES = {torch.float32: _lib.WT_DTYPE_F32, torch.float16: _lib.WT_DTYPE_F16, torch.bfloat16: _lib.WT_DTYPE_BF16}
 _PAGE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.WT_DTYPE_E4M3}
 HEAD_DIMS = (32, 64, 96, 128, 256)
-_current_device = torch.cuda.current_device
 
 
-def _raw_stream(index):
-    return torch.cuda.current_stream(index).cuda_stream
-
-
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)     # (the same handle, without a Stream object around it)
+@functools.lru_cache(maxsize=None)
+def _calls():
+    """The module of the calls, on the entries of the library that ``_lib`` has loaded."""
+    L = _lib.load()
+    try:
+        from . import _kvcalls
+    except ImportError as err:
+        raise ImportError(f"{err}: build it with `make -C {_lib._PKG_ROOT}/csrc`") from err
+    entries = (L.wt_kv_append, L.wt_kv_gather, L.wt_kv_attend, L.wt_kv_attend_workspace, L.wt_last_error)
+    _kvcalls.setup(WtError, *(ctypes.cast(f, ctypes.c_void_p).value for f in entries))
+    return _kvcalls
 
 
 def _overlaps(t):
@@ -87,18 +93,13 @@ class PagedKVCache:
         self.device, self.dtype = k.device, k.dtype
         self.n_pages, self.n_heads, self.page_size, self.head_dim = k.shape
         self.error = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._lib = _lib.load()
-        self._append, self._gather, self._attend = self._lib.wt_kv_append, self._lib.wt_kv_gather, self._lib.wt_kv_attend
-        self._index = self.device.index
-        self._scale = self.head_dim ** -0.5
-
         def strides(t):    # (a dimension of size one has no stride to speak of)
             return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
 
-        self._desc = _lib.KvCache(k.data_ptr(), v.data_ptr(), _lib._ptr(k_exp) or None, _lib._ptr(v_exp) or None, *strides(k), *strides(v),
-                                  self.n_pages, self.n_heads, self.page_size, self.head_dim, _PAGE_DTYPES[k.dtype], 0,
-                                  self.error.data_ptr())
-        self._p = ctypes.addressof(self._desc)
+        desc = _lib.KvCache(k.data_ptr(), v.data_ptr(), _lib._ptr(k_exp) or None, _lib._ptr(v_exp) or None, *strides(k), *strides(v),
+                            self.n_pages, self.n_heads, self.page_size, self.head_dim, _PAGE_DTYPES[k.dtype], 0, self.error.data_ptr())
+        self._calls = _calls()
+        self._handle = self._calls.handle(ctypes.addressof(desc), k)
 
     @classmethod
     def allocate(cls, n_pages: int, n_heads: int, head_dim: int, page_size: int = 64, dtype=torch.float16, device="cuda"):
@@ -109,102 +110,18 @@ class PagedKVCache:
             return cls(k.view(dtype), v.view(dtype), ke, ve)
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
 
-    # --- arguments (a step of a decoder makes two calls a layer: these checks are kept short)
-    def _dtype(self, t_dtype, name):
-        """An 8-bit cache takes and gives any of the three types, another only its own."""
-        dt = _DTYPES.get(t_dtype)
-        if dt is None or (self.k_exp is None and t_dtype is not self.dtype):
-            raise WtError(f"{name}: {t_dtype} with a cache of {self.dtype}")
-        return dt
-
-    def _int32(self, t, name, n):
-        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != self._index or t.shape != (n,) or \
-                not t.is_contiguous():
-            raise WtError(f"{name}: {n} contiguous int32 on {self.device}")
-        return t.data_ptr()
-
-    def _table(self, table):
-        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != self._index:
-            raise WtError(f"page table: int32 (sequences, pages) on {self.device}")
-        n, width = table.shape
-        stride, one = table.stride()
-        if width < 1 or (one != 1 and width > 1) or (n > 1 and stride < width):
-            raise WtError("page table: the pages of a sequence stand side by side, its rows apart")
-        if width * self.page_size > _lib.WT_KV_MAX_POSITIONS:
-            raise WtError(f"page table: {width} pages of {self.page_size} are more than {_lib.WT_KV_MAX_POSITIONS} positions")
-        return table.data_ptr(), stride if n > 1 else width, n, width
-
-    def _rows_of(self, positions, sequences, n_seqs):
-        if not isinstance(positions, torch.Tensor) or positions.dim() != 1:
-            raise WtError("positions: one int32 per row")
-        n = positions.shape[0]
-        pos = self._int32(positions, "positions", n)
-        if sequences is None and n > n_seqs:
-            raise WtError(f"{n} rows for {n_seqs} sequences: say whose they are (sequences=)")
-        return n, None if sequences is None else self._int32(sequences, "sequences", n), pos
-
-    def _new(self, t, name, n):
-        if not isinstance(t, torch.Tensor) or t.get_device() != self._index or t.shape != (n, self.n_heads, self.head_dim):
-            raise WtError(f"{name}: ({n}, {self.n_heads}, {self.head_dim}) on {self.device}")
-        row, head, one = t.stride()
-        row, head = row if n > 1 else 0, head if self.n_heads > 1 else 0
-        p, item = t.data_ptr(), t.element_size()
-        if n and (one != 1 or (p | row * item | head * item) & 15):
-            raise WtError(f"{name}: rows must be contiguous and start on 16-byte steps (strides {t.stride()})")
-        return p, row, head
-
-    def _call(self, entry, *args):
-        """The entry on the current stream of the cache's device -> its return code."""
-        if _current_device() == self._index:
-            return entry(self._p, *args, _raw_stream(self._index))
-        with torch.cuda.device(self.device):
-            return entry(self._p, *args, _raw_stream(self._index))
-
-    # --- operators
+    # --- operators (argument checks, results and launches: csrc/wt_kv_calls.cpp)
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, sequences: torch.Tensor | None = None):
         """Writes rows ``k[r]``, ``v[r]`` (heads, head_dim; any row and head strides of whole 16 bytes) at ``positions[r]``
         of sequence ``sequences[r]`` (None: of sequence r).  A negative position marks a padded row: not written.  No
         two rows of a call may name the same place."""
-        tp, ts, n_seqs, width = self._table(table)
-        n, seq, pos = self._rows_of(positions, sequences, n_seqs)
-        kp, k_row, k_head = self._new(k, "k", n)
-        vp, v_row, v_head = self._new(v, "v", n)
-        if k.dtype is not v.dtype:
-            raise WtError(f"k and v differ: {k.dtype}, {v.dtype}")
-        dt = self._dtype(k.dtype, "k, v")
-        if n:
-            rc = self._call(self._append, kp, vp, dt, k_row, k_head, v_row, v_head, n, tp, ts, n_seqs, width, seq, pos)
-            if rc:
-                _lib._check(rc, "wt_kv_append")
+        self._calls.append(self._handle, k, v, table, positions, sequences)
 
     def gather(self, table: torch.Tensor, positions: torch.Tensor, sequences: torch.Tensor | None = None, dtype=None, out=None):
         """-> (k, v), each (rows, heads, head_dim): the rows at ``positions[r]`` of sequence ``sequences[r]``, in the cache's
         type, or from an 8-bit cache in ``dtype`` (default float32).  A negative position reads as zeros.  ``out``: two
         contiguous tensors to write instead of new ones."""
-        tp, ts, n_seqs, width = self._table(table)
-        n, seq, pos = self._rows_of(positions, sequences, n_seqs)
-        if out is None:
-            if dtype is None:
-                dtype = torch.float32 if self.k_exp is not None else self.dtype
-            dt = self._dtype(dtype, "dtype")
-            k = torch.empty((n, self.n_heads, self.head_dim), dtype=dtype, device=self.device)
-            v = torch.empty_like(k)
-            out = k, v
-        else:
-            k, v = out
-            self._new(k, "out[0]", n), self._new(v, "out[1]", n)
-            if k.dtype is not v.dtype or (dtype is not None and k.dtype is not dtype):
-                raise WtError(f"out: {k.dtype} and {v.dtype}" + (f", not {dtype}" if dtype is not None else ""))
-            dt = self._dtype(k.dtype, "out")
-            if not k.is_contiguous() or not v.is_contiguous():
-                raise WtError("out: not contiguous")
-            if n and k.data_ptr() == v.data_ptr():
-                raise WtError("out: the same memory twice")
-        if n:
-            rc = self._call(self._gather, k.data_ptr(), v.data_ptr(), dt, n, tp, ts, n_seqs, width, seq, pos)
-            if rc:
-                _lib._check(rc, "wt_kv_gather")
-        return out
+        return self._calls.gather(self._handle, table, positions, sequences, dtype, out)
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, scale: float | None = None,
                out: torch.Tensor | None = None, return_lse: bool = False, workspace: torch.Tensor | None = None):
@@ -217,53 +134,12 @@ class PagedKVCache:
         ``workspace`` (from ``attend_workspace``).  Calls that may run at the same time need one each.  A call that is being
         captured into a graph has none of the stream's: without ``workspace`` it takes one in the graph's memory, which
         costs every replay a small kernel that clears its counters."""
-        tp, ts, n_seqs, width = self._table(table)
-        if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.get_device() != self._index:
-            raise WtError(f"q: (sequences, query heads, head_dim) on {self.device}")
-        n, hq, d = q.shape
-        q_row, q_head, one = q.stride()
-        if n != n_seqs or d != self.head_dim or one != 1 or hq < 1 or hq % self.n_heads:
-            raise WtError(f"q: ({n_seqs}, a multiple of {self.n_heads}, {self.head_dim}), a head's values side by side (got {tuple(q.shape)}, "
-                          f"strides {q.stride()})")
-        dt = self._dtype(q.dtype, "q")
-        lp = self._int32(lengths, "lengths", n)
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            o_row, o_head = hq * d, d
-        else:
-            if out.shape != q.shape or out.dtype is not q.dtype or out.device != self.device or out.stride(2) != 1 or _overlaps(out):
-                raise WtError(f"out: {tuple(q.shape)} of {q.dtype} on {self.device}, a head's values side by side, no two in one place")
-            o_row, o_head, _ = out.stride()
-        lse = torch.empty((n, hq), dtype=torch.float32, device=self.device) if return_lse else None
-        if n:
-            wp, w_bytes = None, 0
-            if workspace is not None:
-                if workspace.dtype is not torch.uint8 or workspace.get_device() != self._index or not workspace.is_contiguous():
-                    raise WtError("workspace: what attend_workspace() gave")
-                wp, w_bytes = workspace.data_ptr(), workspace.numel()
-            args = (self._attend, q.data_ptr(), dt, q_row, q_head, n, hq, self._scale if scale is None else scale, tp, ts, width, lp,
-                    out.data_ptr(), o_row, o_head, lse.data_ptr() if return_lse else None)
-            rc = self._call(*args, wp, w_bytes)
-            if rc == _lib.WT_E_CAPTURE and workspace is None:
-                workspace = self.attend_workspace(hq, table)
-                rc = self._call(*args, workspace.data_ptr(), workspace.numel())
-            if rc:
-                _lib._check(rc, "wt_kv_attend")
-        return (out, lse) if return_lse else out
+        return self._calls.attend(self._handle, q, table, lengths, scale, out, return_lse, workspace)
 
     def attend_workspace(self, n_q_heads: int, table: torch.Tensor) -> torch.Tensor | None:
         """A workspace for ``attend`` calls with this many query heads and tables of this shape (or fewer sequences, or fewer
         pages): made ready once, left ready by every call.  None: such calls need none."""
-        _, _, n_seqs, width = self._table(table)
-        with torch.cuda.device(self.device):
-            n = self._lib.wt_kv_attend_workspace(self._p, n_seqs, n_q_heads, width)
-        if n < 0:
-            _lib._check(n, "wt_kv_attend_workspace")
-        if n == 0:
-            return None
-        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
-        ws[:_lib.WT_KV_WORKSPACE_ZEROED].zero_()
-        return ws
+        return self._calls.workspace(self._handle, table, n_q_heads)
 
     def check(self):
         """Waits for the device; raises if a call since the last check met something outside of its range."""
