@@ -485,3 +485,70 @@ def test_offsets_beyond_32_bits():
     want, _, bound, _ = O.attend(q[0].double(), kk.double().cpu(), vv.double().cpu(), 128 ** -0.5)
     assert O.far(out[0], want, bound, BF16) <= 1.0
     cache.check()
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# the path that calls it: B decoder streams with their text in paged caches
+# ----------------------------------------------------------------------------------------------------------------------
+def test_streams_over_paged_caches_match_the_reference(monkeypatch):
+    """transcribe_batch with streams.PAGED_SELF_ATTENTION: ragged prompts, several windows, every recording against the
+    reference's own output at the bars of the concatenated cache; every layer of every call goes through the caches, and
+    the backend is as it was afterwards."""
+    from test_gpu_streams_batch import _check_against_reference
+    from test_streams_host import run_batch, same_model_cases
+    from whisper_timestamped import PagedKVCache, streams
+    calls = {"append": 0, "attend": 0}
+    for name in calls:
+        def counted(self, *a, _f=getattr(PagedKVCache, name), _n=name, **kw):
+            calls[_n] += 1
+            return _f(self, *a, **kw)
+        monkeypatch.setattr(PagedKVCache, name, counted)
+    monkeypatch.setattr(streams, "PAGED_SELF_ATTENTION", True)
+    cases = same_model_cases() + same_model_cases()[::-1]
+    for raw, case in zip(run_batch(cases, device="cuda:0"), cases):
+        _check_against_reference(raw, case)
+    assert calls["attend"] > 50 and calls["append"] > calls["attend"]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_paged_decoder_against_the_backends_own(dtype):
+    """The decoder's logits call by call, over paged caches and over the backend's concatenated ones."""
+    import whisper_double as W
+    from whisper_double.model import build_model
+    from whisper_timestamped.paged_decoder import PagedText, supported
+    W.install()
+    model = build_model("tiny", device="cuda:0")             # (its modules cast their weights to the activations)
+    assert supported(model, dtype)
+    g = torch.Generator().manual_seed(0)
+    feats = torch.randn((3, 1500, 384), generator=g).to(dtype).cuda()
+    prompt = torch.randint(0, 50000, (3, 11), generator=g).cuda()
+    steps = torch.randint(0, 50000, (3, 40), generator=g).cuda()
+
+    def logits():
+        cache, hooks = model.install_kv_cache_hooks()
+        try:
+            with torch.no_grad():
+                out = [model.decoder(prompt, feats, kv_cache=cache)[:, -1:]]
+                for i in range(steps.shape[1]):
+                    out.append(model.decoder(steps[:, i:i + 1], feats, kv_cache=cache))
+        finally:
+            for h in hooks:
+                h.remove()
+        return torch.cat(out, 1)
+
+    want = logits()
+    text = PagedText(model, 4, dtype)
+    for _ in range(2):                                   # (a second loop starts from empty caches)
+        with text.attached():
+            got = logits()
+        # attention in 32 bits against the backend's in the model's type: layer by layer a few roundings of the residual
+        # stream apart, 4 layers, logits of standard deviation ~ 10; f32 2^-24, f16 2^-11 a rounding
+        tol = (1e-3 if dtype == torch.float32 else 0.5)
+        assert float((got - want).abs().max()) <= tol
+    assert "forward" not in vars(model.decoder.blocks[0].attn) and "install_kv_cache_hooks" not in vars(model)
+    assert torch.equal(logits(), want)
+    for c in text.caches:
+        c.check()
+    from whisper_timestamped._lib import WtError
+    with text.attached(), pytest.raises(WtError, match="room for 4"):
+        model.decoder(prompt[:1].repeat(5, 1), feats[:1].repeat(5, 1, 1), kv_cache=model.install_kv_cache_hooks()[0])

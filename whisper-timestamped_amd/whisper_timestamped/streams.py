@@ -43,6 +43,7 @@ through the batch size of the backend's GEMMs (tests: B = 8 equals eight B = 1 r
 """
 from __future__ import annotations
 
+import contextlib
 import logging
 import threading
 
@@ -67,6 +68,11 @@ LAST_RUN = {}
 #  profiles/r5f_bench_driver_command.json `ragged_bucket_admission` keeps the record.)
 PAUSE_GC = True               # pause Python's cyclic garbage collector while a batch decodes (see _run_streams)
 GC_EVERY_ROUNDS = 8           # ... with a young-generation pass every this many rounds (a long batch must not hoard cycles)
+
+
+# The decoder's self-attention over paged caches (paged_decoder.py) instead of the backend's concatenated ones.  Off by default:
+# its sums are in another order than the backend's, so results agree to rounding, not bit for bit.
+PAGED_SELF_ATTENTION = False
 
 
 class paused_gc:
@@ -859,6 +865,13 @@ def _run_streams(model, audios, opts, max_streams, **session_kwargs):
     loop_sizes = []
     verify = efficient.REUSE_DECODER_LOGITS == "auto"
     fused_checked = False
+    text = None
+    if PAGED_SELF_ATTENTION:
+        from . import paged_decoder
+        if paged_decoder.supported(model, dtype):
+            text = paged_decoder.PagedText(model, S, dtype)
+        else:
+            logger.warning("whisper_timestamped: PAGED_SELF_ATTENTION does not know this backend's attention modules; its own cache is used")
     # The driver's loops allocate a few thousand small ACYCLIC objects per stream and window (token lists, word dictionaries,
     # views): reference counting frees them; the cyclic collector only re-scans the process's long-lived objects (the model's
     # modules, torch's own tables) every few thousand allocations -- a tenth of a 256-stream loop's host time
@@ -914,7 +927,8 @@ def _run_streams(model, audios, opts, max_streams, **session_kwargs):
                     try:
                         feats = task._get_audio_features(mel_batch[members])
                         tokens0 = torch.tensor([st.initial_tokens for st in grp], device=dev)
-                        tokens, sum_logprobs, no_speech = task._main_loop(feats, tokens0)
+                        with text.attached() if text is not None else contextlib.nullcontext():
+                            tokens, sum_logprobs, no_speech = task._main_loop(feats, tokens0)
                         rec.commit(tokens[:, -1], final=True)  # the last call's rows and what was sampled from them
                     finally:
                         rec.remove()
