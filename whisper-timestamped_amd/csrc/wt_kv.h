@@ -115,7 +115,8 @@ struct KvAttend {
     float *lse;
     bool q_aligned, o_aligned;       // every row of q starts on 16 bytes; of out, on four elements
     // schedule
-    int direct;                      // 1: one workgroup per (sequence, key head, tile), 2: one wave; no workspace
+    int direct;                      // one workgroup per (sequence, key head, tile), no workspace
+    int waves;                       // of a workgroup: KV_WAVES, or 2
     int n_wg, min_share, seg_cost;
     int32_t *counters;               // 4 * n_wg, zero between calls
     float *partials;                 // 2 * n_wg slots: maxima and sums of 16 queries, the same of a joined group, sums of values

@@ -302,7 +302,7 @@ int kv_attend_e4m3_bf16(const KvAttend &, unsigned, hipStream_t);
 __global__ void kv_zero_kernel(int32_t *p) { p[blockIdx.x * 256 + threadIdx.x] = 0; }
 
 struct KvPlan {
-    int direct, n_wg, min_share, seg_cost;
+    int direct, waves, n_wg, min_share, seg_cost;
     unsigned grid;
     int64_t bytes;
 };
@@ -323,12 +323,14 @@ static int kv_plan(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_wi
     p->min_share = 4;
     p->seg_cost = 2;
     // One workgroup streams 512 KB of keys and values in about the time that splitting them costs (measured, 8 to 640 pairs in
-    // four types: 256 KB 9.6 us against 13.3, 512 KB 13.9 against 14.7, 1 MB 27.6 against 16.2).  With as many pairs as keep
-    // every wave slot busy, a wave each is better still: 5120 pairs of 32 / 128 / 448 keys 15.6 / 33.7 / 94.7 us against 17.8 /
-    // 50.0 / 113; 768 pairs of 256 keys 13.1 against 13.4, of 448 19.7 against 19.3.
+    // four types: 256 KB 9.6 us against 13.3, 512 KB 13.9 against 14.7, 1 MB 27.6 against 16.2).
     p->direct = (int64_t)table_width * c->page_size * key_bytes <= 512 * 1024;
-    if (p->direct && pairs >= 8 * n) p->direct = 2;
-    p->grid = p->direct == 0 ? (unsigned)p->n_wg : p->direct == 1 ? (unsigned)pairs : (unsigned)((pairs + 3) / 4);
+    // Where the pairs fill the card by themselves, workgroups of two waves let more of them run at once.  Four / two waves, us:
+    // f16, 64 values, 256 pairs of 1..448 keys 6.6 / 7.2, 512 9.4 / 8.7, 1536 17.6 / 15.0, 5120 44.4 / 36.1; bf16, 128 values, 768 of 448
+    // 35.4 / 31.7; f32, 768 of 10..1000 34.8 / 38.6, 1536 of 1..448 27.5 / 24.1; 8 bits, 1536 of 10..1000 18.2 / 21.3, 5120 of 1..448 26.0 /
+    // 23.0.  (One wave: 5120 pairs of 128 keys each 32.9 against 39.8 with two, but of 1..448 keys 44.6 against 36.1.)
+    p->waves = p->direct && pairs >= n * (c->dtype == WT_DTYPE_F32 ? 6 : c->dtype == WT_DTYPE_E4M3 ? 12 : 2) ? 2 : KV_WAVES;
+    p->grid = p->direct ? (unsigned)pairs : (unsigned)p->n_wg;
     p->bytes = p->direct ? 0 : WT_KV_WORKSPACE_ZEROED + (int64_t)p->n_wg * 2 * kv_slot(c->head_dim) * 4;
     return WT_OK;
 }
@@ -397,7 +399,7 @@ int kv_attend(const wt_kv_cache *c, const void *q, int dtype, int64_t q_row, int
     a.scale = scale, a.lengths = lengths, a.out = out, a.o_row = o_row, a.o_head = o_head, a.lse = lse;
     a.q_aligned = (((uintptr_t)q | (uint64_t)(q_row * item) | (uint64_t)(q_head * item)) & 15) == 0;
     a.o_aligned = (((uintptr_t)out | (uint64_t)(o_row * item) | (uint64_t)(o_head * item)) & (4 * item - 1)) == 0;
-    a.direct = p.direct, a.n_wg = p.n_wg, a.min_share = p.min_share, a.seg_cost = p.seg_cost;
+    a.direct = p.direct, a.waves = p.waves, a.n_wg = p.n_wg, a.min_share = p.min_share, a.seg_cost = p.seg_cost;
     a.counters = (int32_t *)workspace;
     a.partials = workspace ? (float *)((char *)workspace + WT_KV_WORKSPACE_ZEROED) : nullptr;
     if (c->dtype == WT_DTYPE_E4M3)

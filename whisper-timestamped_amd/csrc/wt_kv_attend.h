@@ -636,61 +636,13 @@ __device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, in
     }
 }
 
-// Short tables: one workgroup of NW waves per (sequence, key head, query tile); one wave, four pairs a workgroup, where a
-// pair's keys are few or the pairs many.
+// Short tables: one workgroup per (sequence, key head, query tile).
 template <typename CT, typename T, int HD, int PG, int NW>
 __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_direct_kernel(const KvAttend a) {
     extern __shared__ __attribute__((aligned(16))) float kv_lds[];
     const unsigned pairs = a.c.n_heads * a.q_tiles;
     KvWave<CT, T, HD, PG, NW> w(a);
     kv_segment<true, CT, T, HD, PG, NW>(w, a, kv_lds, blockIdx.x / pairs, blockIdx.x % pairs, 0, false, 0, 0, -1);
-}
-
-template <typename CT, typename T, int HD, int PG>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void kv_attend_wave_kernel(const KvAttend a) {
-    constexpr int EV = HD / 16, KB = KvKind<CT, T, HD>::KB;
-    const unsigned pairs = a.c.n_heads * a.q_tiles;
-    const unsigned at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int s = at / pairs, pair = at % pairs;
-    if (s >= a.t.n_seqs) return;
-    const int h = pair / a.q_tiles, qt = pair % a.q_tiles;
-    const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
-    KvWave<CT, T, HD, PG, 1> w(a);
-    w.row = a.t.t + s * a.t.stride;
-    w.h = h;
-    typename KvWave<CT, T, HD, PG, 1>::Raw raw;
-    const int raw_len = a.lengths[s];
-    const auto first = w.ids(0, (int)kv_capacity(a));
-    w.queries_load(raw, s, hq0, rows);
-    bool bad_len;
-    const int len = __builtin_amdgcn_readfirstlane(kv_length(a, raw_len, &bad_len));
-    w.len = len;
-    w.bad = bad_len;
-    w.run(0, (len + KB - 1) / KB, first, raw, rows);
-    const bool bad = __any(w.bad);
-    if (bad && w.lane == 0) kv_report(a.c.error, bad_len ? WT_KV_BAD_POSITION : WT_KV_BAD_PAGE);
-    float l = w.l;
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (bad) l = __builtin_nanf("");
-    const bool empty = len == 0 && !bad_len;
-    if (w.n < rows) {
-        constexpr int C = EV % 4 == 0 ? 4 : 2;
-        const float inv = empty ? 0.f : 1.f / l;
-        T *dst = static_cast<T *>(a.out) + s * a.o_row + (hq0 + w.n) * a.o_head + w.g * 4 * EV;
-#pragma unroll
-        for (int e = 0; e < 4 * EV; e += C) {
-            Pack<T, C> v;
-#pragma unroll
-            for (int x = 0; x < C; ++x) v.v[x] = from_f<T>(empty ? 0.f : w.o[(e + x) % EV][(e + x) / EV] * inv);
-            if (a.o_aligned) *reinterpret_cast<Pack<T, C> *>(dst + e) = v;
-            else {
-#pragma unroll
-                for (int x = 0; x < C; ++x) dst[e + x] = v.v[x];
-            }
-        }
-        if (a.lse && w.g == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + w.n] = empty ? -__builtin_inff() : w.m + logf(l);
-    }
 }
 
 template <typename CT, typename T, int HD, int PG, int NW>
@@ -771,17 +723,15 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_kernel(c
 
 template <typename CT, typename T, int HD, int PG>
 static int kv_attend_go(const KvAttend &a, unsigned grid, hipStream_t st) {
-    constexpr int NW = KV_WAVES;
     const int rows = a.group < 16 ? a.group : 16;
-    size_t lds = sizeof(float) * NW * (32 + (size_t)rows * HD);
-    if (lds < sizeof(float) * NW * 64 * 6) lds = sizeof(float) * NW * 64 * 6;   // what the join of partial results takes
-    const auto kernel = a.direct == 0   ? kv_attend_kernel<CT, T, HD, PG, NW>
-                        : a.direct == 1 ? kv_attend_direct_kernel<CT, T, HD, PG, NW>
-                                        : kv_attend_wave_kernel<CT, T, HD, PG>;
-    if (a.direct == 2) lds = 0;
+    void (*kernel)(KvAttend) = !a.direct     ? kv_attend_kernel<CT, T, HD, PG, KV_WAVES>
+                               : a.waves == 2 ? kv_attend_direct_kernel<CT, T, HD, PG, 2>
+                                              : kv_attend_direct_kernel<CT, T, HD, PG, KV_WAVES>;
+    size_t lds = sizeof(float) * a.waves * (32 + (size_t)rows * HD);
+    if (!a.direct && lds < sizeof(float) * KV_WAVES * 64 * 6) lds = sizeof(float) * KV_WAVES * 64 * 6;   // what the join of partial results takes
     if (lds > 64 * 1024)   // (16 queries of 256 values)
         WT_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * a.waves), lds, st, a);
     WT_HIP(hipGetLastError());
     return WT_OK;
 }
