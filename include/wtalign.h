@@ -327,7 +327,7 @@ typedef struct wt_kv_cache {
     int32_t *error;
 } wt_kv_cache;
 
-/* Writes n_rows new rows: row r is position positions[r] of sequence sequences[r] (NULL: of sequence r; then
+/* Writes n_rows (at most 2^30) new rows: row r is position positions[r] of sequence sequences[r] (NULL: of sequence r; then
  * n_rows <= n_seqs).  A row of negative position is a padded one: not written.  No two rows of a call may name the same
  * place.  Slots that no row names keep what they hold.
  *   k, v : device, element d of head h of row r at k[r * k_row_stride + h * k_head_stride + d]; multiples of 16 bytes;

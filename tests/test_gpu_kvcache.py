@@ -131,6 +131,45 @@ def test_attend_many_short_sequences(q_dtype, dtype):
     check_attend([(7 * i) % 40 for i in range(150)], 1, 6, 32, 8, q_dtype, dtype, seed=9)
 
 
+@pytest.mark.parametrize("group,heads,width,q_dtype,dtype", [(1, 2, 128, BF16, BF16), (17, 1, 64, F32, F32), (20, 1, 96, F16, E4M3), (2, 1, 256, F16, F16), (3, 2, 32, BF16, E4M3)])
+def test_attend_shares_of_many_sequences(group, heads, width, q_dtype, dtype):
+    """Long tables over more sequences than a wave has lanes: empty ones at every place where the prefix sums change hands,
+    ones of a single key, some that many workgroups share."""
+    lengths = [(i * 37) % 90 for i in range(150)]
+    for i in (0, 62, 63, 64, 127, 128, 149):
+        lengths[i] = 0
+    item = {F32: 4, E4M3: 1}.get(dtype, 2)
+    long = 600000 // (2 * width * item)                  # beyond what one workgroup takes by itself
+    lengths[1], lengths[65], lengths[66], lengths[148] = long, 3 * long + 1, 1, 2 * long - 3
+    check_attend(lengths, group, heads, width, 16, q_dtype, dtype, seed=group)
+
+
+def test_attend_shares_of_empty_sequences():
+    cache, table, _, _, _ = make([0] * 70, 2, 64, 16, F16)
+    wide = torch.zeros((70, 5000), dtype=torch.int32, device=DEV)
+    out, lse = cache.attend(queries(70, 2, 64, F16, 0).to(DEV), wide, torch.zeros(70, dtype=torch.int32, device=DEV), return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    cache.check()
+
+
+def test_attend_workspace():
+    """One workspace for calls of different shapes, one after the other; another's size, type or device is refused."""
+    from whisper_timestamped._lib import WtError
+    cache, table, _, _, _ = make([4000, 3, 2500], 2, 64, 16, F16, seed=5)
+    lens = torch.tensor([4000, 3, 2500], dtype=torch.int32, device=DEV)
+    ws = cache.attend_workspace(8, table)
+    assert ws is not None and cache.attend_workspace(8, table[:, :16]) is None
+    for heads in (8, 2, 8, 4):
+        q = queries(3, heads, 64, F16, heads).to(DEV)
+        want = cache.attend(q, table, lens)
+        assert torch.equal(cache.attend(q, table, lens, workspace=ws), want)
+        assert torch.equal(cache.attend(q[:2], table[:2], lens[:2], workspace=ws), want[:2])
+    assert bool((ws[:16384] == 0).all()), "a call leaves the counters at zero"
+    for bad in (ws[:20000], ws.view(torch.int32), ws.cpu(), ws[1:]):
+        with pytest.raises(WtError, match="workspace"):
+            cache.attend(q, table, lens, workspace=bad)
+
+
 @pytest.mark.parametrize("q_dtype,dtype", PAIRS)
 @pytest.mark.parametrize("scale,q_gain", [(1.0, 4.0), (-0.5, 1.0), (0.0, 1.0), (1e-3, 1.0)])
 def test_attend_scales(q_dtype, dtype, scale, q_gain):

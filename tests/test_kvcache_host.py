@@ -30,6 +30,13 @@ def pages(*shape, dtype=torch.float16):
     (pages(4, 2, 16, 64, dtype=E4M3), pages(4, 2, 16, 64, dtype=E4M3), pages(4, 2, 15, dtype=torch.uint8), pages(4, 2, 16, dtype=torch.uint8), "k_exp"),
     (pages(4, 2, 16, 64, dtype=E4M3), pages(4, 2, 16, 64, dtype=E4M3), pages(4, 2, 16, dtype=torch.uint8), pages(4, 2, 16), "v_exp"),
     (pages(4, 2, 16, 64), pages(4, 2, 16, 64), None, None, "GPU"),
+    (pages(4, 2, 16, 64).transpose(0, 2), pages(4, 2, 16, 64).transpose(0, 2), None, None, "GPU"),
+    (pages(4, 2, 16, 128)[..., :64], pages(4, 2, 16, 128)[..., 64:], None, None, "GPU"),
+    (torch.zeros(9000, dtype=torch.float16).as_strided((4, 2, 16, 64), (128, 64, 512, 1)), pages(4, 2, 16, 64), None, None, "GPU"),
+    (torch.zeros(9000, dtype=torch.float16).as_strided((4, 2, 16, 64), (1024, 1024, 64, 1)), pages(4, 2, 16, 64), None, None, "overlap"),
+    ([1], pages(4, 2, 16, 64), None, None, "k: not a tensor"),
+    (pages(1, 70000, 1, 32), pages(1, 70000, 1, 32), None, None, "65535 heads"),
+    (pages(4, 2, 16, 64, dtype=E4M3), pages(4, 2, 16, 64, dtype=E4M3), pages(4, 2, 16, dtype=torch.uint8), pages(4, 2, 17, dtype=torch.uint8).reshape(-1)[1:129].view(4, 2, 16), "16-byte aligned"),
 ])
 def test_construction(k, v, ke, ve, said):
     with pytest.raises(WtError, match=said):
@@ -44,6 +51,12 @@ def test_the_same_memory_twice():
 
 # The C entries check on the host before they launch: made-up addresses never reach the device.
 A = 1 << 20
+
+
+def test_the_same_exponents_twice():
+    k, v, e = pages(4, 2, 16, 64, dtype=E4M3), pages(4, 2, 16, 64, dtype=E4M3), pages(4, 2, 16, dtype=torch.uint8)
+    with pytest.raises(WtError, match="k_exp and v_exp are the same memory"):
+        PagedKVCache(k, v, e, e)
 
 
 def desc(**kw):
@@ -71,7 +84,7 @@ def attend(c=None, **kw):
     return _lib.load().wt_kv_attend(ctypes.byref(c or desc()), *a.values())
 
 
-BAD_CACHES = [dict(k=None), dict(v=None), dict(n_pages=0), dict(n_heads=0), dict(page_size=0), dict(reserved=1), dict(dtype=4), dict(dtype=0), dict(k=A + 8),
+BAD_CACHES = [dict(k=None), dict(v=None), dict(n_pages=0), dict(n_heads=0), dict(n_heads=65536), dict(page_size=0), dict(reserved=1), dict(dtype=4), dict(dtype=0), dict(k=A + 8),
               dict(k_exp=A), dict(dtype=3), dict(k_slot_stride=65), dict(v_head_stride=-64), dict(head_dim=80), dict(head_dim=0)]
 
 
@@ -82,7 +95,7 @@ def test_entries_refuse_a_bad_cache(bad):
         assert b"wt_kv_" in _lib.load().wt_last_error()
 
 
-@pytest.mark.parametrize("bad", [dict(k=None), dict(v=A + 2), dict(k=A + 8), dict(dtype=0), dict(dtype=3), dict(k_row=130), dict(v_head=4), dict(n_rows=-1),
+@pytest.mark.parametrize("bad", [dict(k=None), dict(v=A + 2), dict(k=A + 8), dict(dtype=0), dict(dtype=3), dict(k_row=130), dict(v_head=4), dict(n_rows=-1), dict(n_rows=(1 << 30) + 1, seq=A),
                                  dict(n_rows=3), dict(pos=None), dict(table=None), dict(stride=3), dict(width=0), dict(width=1 << 28), dict(n_seqs=-1)],
                          ids=lambda b: ",".join(f"{k}={v}" for k, v in b.items()))
 def test_append_refuses(bad):
@@ -116,12 +129,11 @@ def test_cache_descriptor_matches_the_header():
 def host_cache(dtype=torch.float16, heads=2, page=16, width=64):
     from whisper_timestamped import kvcache
     cache = object.__new__(PagedKVCache)
-    cache.k, cache.v = pages(4, heads, page, width, dtype=dtype), pages(4, heads, page, width, dtype=dtype)
-    e = pages(4, heads, page, dtype=torch.uint8).data_ptr() if dtype == E4M3 else None
-    cache._keep = desc(k=cache.k.data_ptr(), v=cache.v.data_ptr(), k_exp=e, v_exp=e, n_heads=heads, page_size=page, head_dim=width,
-                       dtype=kvcache._PAGE_DTYPES[dtype])
+    k, v = pages(4, heads, page, width, dtype=dtype), pages(4, heads, page, width, dtype=dtype)
+    e = [pages(4, heads, page, dtype=torch.uint8) if dtype == E4M3 else None for _ in range(2)]
     cache._calls = kvcache._calls()
-    cache._handle = cache._calls.handle(ctypes.addressof(cache._keep), cache.k)
+    cache._handle, cache.error = cache._calls.make(k, v, *e, True)
+    cache._keep = k, v, e
     return cache
 
 
@@ -209,6 +221,21 @@ def test_attend_arguments(change, said):
     a = dict(q=Q, table=TABLE, lengths=i32(1, 2, 3))
     with pytest.raises(WtError, match=said):
         host_cache().attend(**dict(a, **change))
+
+
+def test_gradients_are_refused():
+    """Recorded calls would silently lack their gradient; under no_grad the same tensors are taken."""
+    w = [pages(3, 2, 64).requires_grad_() for _ in range(2)]
+    q = Q.clone().requires_grad_()
+    c = host_cache()
+    for f in (lambda: c.append(w[0], ROWS, TABLE, i32(0, 1, 2)), lambda: c.append(ROWS, w[1], TABLE, i32(0, 1, 2)), lambda: c.attend(q, TABLE, i32(1, 2, 3)),
+              lambda: c.attend(Q, TABLE, i32(1, 2, 3), out=q), lambda: c.gather(TABLE, i32(0, 1, 2), out=tuple(w))):
+        with pytest.raises(WtError, match="gradient"):
+            f()
+        with torch.no_grad(), pytest.raises(WtError, match="only run on the GPU"):
+            f()
+    with pytest.raises(WtError, match="no gradient"):
+        PagedKVCache(pages(4, 2, 16, 64).requires_grad_(), pages(4, 2, 16, 64))
 
 
 def test_attend_wrong_python_types():

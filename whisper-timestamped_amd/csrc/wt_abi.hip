@@ -73,15 +73,19 @@ int scratch_tagged(hipStream_t st, size_t bytes, void **out, const void *tag_ptr
     a->tag_val = tag_val;
     return WT_OK;
 }
-// workspace of wt_kv_attend; `fresh`: new memory, whose counters the caller has to clear on `st`
-int scratch_kv(hipStream_t st, size_t bytes, void **out, bool *fresh) {
+// Workspace of wt_kv_attend, always of the same size: it never grows, so that what one call was given no other call frees.
+// New memory is cleared (queued on `st`) before any other call can be given it.
+int kv_clear(void *workspace, hipStream_t st);
+int scratch_kv(hipStream_t st, size_t bytes, void **out) {
+    static std::mutex mu;
+    std::lock_guard<std::mutex> one(mu);
     Arena *a = nullptr;
-    const int rc = scratch_ex(3, st, bytes, out, &a);
-    if (rc) return rc;
-    std::lock_guard<std::mutex> lk(g_mu);
-    *fresh = a->tag_val != 1;
-    a->tag_val = 1;
-    return WT_OK;
+    int rc = scratch_ex(3, st, bytes, out, &a);
+    if (rc == WT_OK && a->tag_val != 1) {
+        rc = kv_clear(*out, st);
+        if (rc == WT_OK) a->tag_val = 1;
+    }
+    return rc;
 }
 void scratch_forget_tags() {
     std::lock_guard<std::mutex> lk(g_mu);

@@ -20,6 +20,7 @@ struct RowSplit {
     static constexpr int HPW = GROUPS / RPW;
 };
 constexpr int KV_HU = 4;
+constexpr int KV_MAX_ROWS = 1 << 25;   // rows of one launch (4 a workgroup at least, a grid has less than 2^32 threads)
 
 template <int N>   // N bytes as the widest loads and stores their alignment allows
 struct Bytes {
@@ -69,12 +70,12 @@ __device__ __forceinline__ void kv_quantise(const Bytes<EPL * sizeof(ST)> &src, 
 template <typename ST, typename CT, int HD>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvRows k, KvRows v, KvDims c, KvTable t, const ST *__restrict__ ks,
                                                         const ST *__restrict__ vs, int64_t k_row, int64_t k_head, int64_t v_row,
-                                                        int64_t v_head, int n_rows, const int32_t *__restrict__ sequences,
+                                                        int64_t v_head, int row0, int n_rows, const int32_t *__restrict__ sequences,
                                                         const int32_t *__restrict__ positions) {
     using R = RowSplit<ST, HD>;
     constexpr int EPL = R::EPL;
     const int g = threadIdx.x / R::LPR, lane = threadIdx.x % R::LPR;
-    const int r = blockIdx.x * R::RPW + g % R::RPW, h0 = blockIdx.y * R::HPW * KV_HU + g / R::RPW;
+    const int r = row0 + blockIdx.x * R::RPW + g % R::RPW, h0 = blockIdx.y * R::HPW * KV_HU + g / R::RPW;
     if (g >= R::GROUPS || r >= n_rows) return;   // whole lane groups
     const int pos = positions[r];
     Bytes<EPL * sizeof(ST)> kr[KV_HU], vr[KV_HU];
@@ -130,12 +131,12 @@ __device__ __forceinline__ void kv_emit(const Bytes<EPL * sizeof(CT)> &src, uint
 
 template <typename DT, typename CT, int HD>
 __global__ __launch_bounds__(256) void kv_gather_kernel(KvRows k, KvRows v, KvDims c, KvTable t, DT *__restrict__ kd,
-                                                        DT *__restrict__ vd, int n_rows, const int32_t *__restrict__ sequences,
+                                                        DT *__restrict__ vd, int row0, int n_rows, const int32_t *__restrict__ sequences,
                                                         const int32_t *__restrict__ positions) {
     using R = RowSplit<DT, HD>;
     constexpr int EPL = R::EPL;
     const int g = threadIdx.x / R::LPR, lane = threadIdx.x % R::LPR;
-    const int r = blockIdx.x * R::RPW + g % R::RPW, h0 = blockIdx.y * R::HPW * KV_HU + g / R::RPW;
+    const int r = row0 + blockIdx.x * R::RPW + g % R::RPW, h0 = blockIdx.y * R::HPW * KV_HU + g / R::RPW;
     if (g >= R::GROUPS || r >= n_rows) return;
     const int pos = positions[r];
     int page = 0, slot = 0;
@@ -168,8 +169,8 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvRows k, KvRows v, KvDi
 // ---- host -----------------------------------------------------------------------------------------------------------
 static int kv_check(const char *what, const wt_kv_cache *c, int dtype, const int32_t *table, int64_t table_stride, int n_seqs,
                     int table_width) {
-    if (!c || !c->k || !c->v || c->n_pages <= 0 || c->n_heads <= 0 || c->page_size <= 0 || c->reserved != 0) {
-        set_error("%s: null cache or pages, or a size below one", what);
+    if (!c || !c->k || !c->v || c->n_pages <= 0 || c->n_heads <= 0 || c->n_heads > 65535 || c->page_size <= 0 || c->reserved != 0) {
+        set_error("%s: null cache or pages, a size below one, or more than 65535 heads", what);
         return WT_E_BADARG;
     }
     if (c->dtype < WT_DTYPE_F32 || c->dtype > WT_DTYPE_E4M3 || dtype < WT_DTYPE_F32 || dtype > WT_DTYPE_BF16 ||
@@ -217,7 +218,7 @@ static KvDims kv_dims(const wt_kv_cache *c) {
 
 static int kv_check_rows(const char *what, const void *k, const void *v, int n_rows, int n_seqs, const int32_t *sequences,
                          const int32_t *positions) {
-    if (!k || !v || !positions || n_rows < 0 || (!sequences && n_rows > n_seqs)) {
+    if (!k || !v || !positions || n_rows < 0 || n_rows > (1 << 30) || (!sequences && n_rows > n_seqs)) {
         set_error("%s: null pointer, or %d rows for %d sequences", what, n_rows, n_seqs);
         return WT_E_BADARG;
     }
@@ -264,14 +265,17 @@ int kv_append(const wt_kv_cache *c, const void *k, const void *v, int dtype, int
         return WT_E_BADARG;
     }
     if (n_rows == 0) return WT_OK;
-#define WT_KV_GO(ST, CT, HD)                                                                                                     \
-    hipLaunchKernelGGL((kv_append_kernel<ST, CT, HD>), (kv_row_grid<ST, HD>(n_rows, c->n_heads)), dim3(256), 0, st, kv_k(c), kv_v(c), \
-                       kv_dims(c), (KvTable{table, table_stride, n_seqs, table_width}), (const ST *)k, (const ST *)v, k_row, k_head,   \
-                       v_row, v_head, n_rows, sequences, positions)
+#define WT_KV_GO(ST, CT, HD)                                                                                                   \
+    hipLaunchKernelGGL((kv_append_kernel<ST, CT, HD>), (kv_row_grid<ST, HD>(end - r0, c->n_heads)), dim3(256), 0, st, kv_k(c), kv_v(c), \
+                       kv_dims(c), (KvTable{table, table_stride, n_seqs, table_width}), (const ST *)k, (const ST *)v, k_row, k_head, v_row, \
+                       v_head, r0, end, sequences, positions)
 #define WT_KV_M(F, A, B) WT_KV_WIDTHS(F, A, B)
-    WT_KV_TYPES(WT_KV_M, WT_KV_GO)
+    for (int64_t r = 0; r < n_rows; r += KV_MAX_ROWS) {
+        const int r0 = (int)r, end = (int)(r + KV_MAX_ROWS < n_rows ? r + KV_MAX_ROWS : n_rows);
+        WT_KV_TYPES(WT_KV_M, WT_KV_GO)
+        WT_HIP(hipGetLastError());
+    }
 #undef WT_KV_GO
-    WT_HIP(hipGetLastError());
     return WT_OK;
 }
 
@@ -281,17 +285,20 @@ int kv_gather(const wt_kv_cache *c, void *k, void *v, int dtype, int n_rows, con
     if (!rc) rc = kv_check_rows("wt_kv_gather", k, v, n_rows, n_seqs, sequences, positions);
     if (rc) return rc;
     if (n_rows == 0) return WT_OK;
-#define WT_KV_GO(DT, CT, HD)                                                                                                     \
-    hipLaunchKernelGGL((kv_gather_kernel<DT, CT, HD>), (kv_row_grid<DT, HD>(n_rows, c->n_heads)), dim3(256), 0, st, kv_k(c), kv_v(c), \
-                       kv_dims(c), (KvTable{table, table_stride, n_seqs, table_width}), (DT *)k, (DT *)v, n_rows, sequences, positions)
-    WT_KV_TYPES(WT_KV_M, WT_KV_GO)
+#define WT_KV_GO(DT, CT, HD)                                                                                                   \
+    hipLaunchKernelGGL((kv_gather_kernel<DT, CT, HD>), (kv_row_grid<DT, HD>(end - r0, c->n_heads)), dim3(256), 0, st, kv_k(c), kv_v(c), \
+                       kv_dims(c), (KvTable{table, table_stride, n_seqs, table_width}), (DT *)k, (DT *)v, r0, end, sequences, positions)
+    for (int64_t r = 0; r < n_rows; r += KV_MAX_ROWS) {
+        const int r0 = (int)r, end = (int)(r + KV_MAX_ROWS < n_rows ? r + KV_MAX_ROWS : n_rows);
+        WT_KV_TYPES(WT_KV_M, WT_KV_GO)
+        WT_HIP(hipGetLastError());
+    }
 #undef WT_KV_GO
-    WT_HIP(hipGetLastError());
     return WT_OK;
 }
 
 // ---- attention of one new token: schedule ------------------------------------------------------------------------------
-int scratch_kv(hipStream_t st, size_t bytes, void **out, bool *fresh);
+int scratch_kv(hipStream_t st, size_t bytes, void **out);
 int kv_attend_f32(const KvAttend &, unsigned, hipStream_t);
 int kv_attend_f16(const KvAttend &, unsigned, hipStream_t);
 int kv_attend_bf16(const KvAttend &, unsigned, hipStream_t);
@@ -300,6 +307,14 @@ int kv_attend_e4m3_f16(const KvAttend &, unsigned, hipStream_t);
 int kv_attend_e4m3_bf16(const KvAttend &, unsigned, hipStream_t);
 
 __global__ void kv_zero_kernel(int32_t *p) { p[blockIdx.x * 256 + threadIdx.x] = 0; }
+int kv_clear(void *workspace, hipStream_t st) {
+    hipLaunchKernelGGL(kv_zero_kernel, dim3(WT_KV_WORKSPACE_ZEROED / 1024), dim3(256), 0, st, (int32_t *)workspace);
+    WT_HIP(hipGetLastError());
+    return WT_OK;
+}
+static int64_t kv_workspace(int n_wg, int head_dim) { return WT_KV_WORKSPACE_ZEROED + (int64_t)n_wg * 2 * kv_slot(head_dim) * 4; }
+
+constexpr int64_t KV_MAX_GRID = 1 << 23;   // workgroups of one launch: a grid has less than 2^32 threads
 
 struct KvPlan {
     int direct, waves, n_wg, min_share, seg_cost;
@@ -324,14 +339,14 @@ static int kv_plan(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_wi
     p->seg_cost = 2;
     // One workgroup streams 512 KB of keys and values in about the time that splitting them costs (measured, 8 to 640 pairs in
     // four types: 256 KB 9.6 us against 13.3, 512 KB 13.9 against 14.7, 1 MB 27.6 against 16.2).
-    p->direct = (int64_t)table_width * c->page_size * key_bytes <= 512 * 1024;
+    p->direct = (int64_t)table_width * c->page_size * key_bytes <= 512 * 1024 && pairs <= KV_MAX_GRID;
     // Where the pairs fill the card by themselves, workgroups of two waves let more of them run at once.  Four / two waves, us:
     // f16, 64 values, 256 pairs of 1..448 keys 6.6 / 7.2, 512 9.4 / 8.7, 1536 17.6 / 15.0, 5120 44.4 / 36.1; bf16, 128 values, 768 of 448
     // 35.4 / 31.7; f32, 768 of 10..1000 34.8 / 38.6, 1536 of 1..448 27.5 / 24.1; 8 bits, 1536 of 10..1000 18.2 / 21.3, 5120 of 1..448 26.0 /
     // 23.0.  (One wave: 5120 pairs of 128 keys each 32.9 against 39.8 with two, but of 1..448 keys 44.6 against 36.1.)
     p->waves = p->direct && pairs >= n * (c->dtype == WT_DTYPE_F32 ? 6 : c->dtype == WT_DTYPE_E4M3 ? 12 : 2) ? 2 : KV_WAVES;
     p->grid = p->direct ? (unsigned)pairs : (unsigned)p->n_wg;
-    p->bytes = p->direct ? 0 : WT_KV_WORKSPACE_ZEROED + (int64_t)p->n_wg * 2 * kv_slot(c->head_dim) * 4;
+    p->bytes = p->direct ? 0 : kv_workspace(p->n_wg, c->head_dim);
     return WT_OK;
 }
 
@@ -387,9 +402,7 @@ int kv_attend(const wt_kv_cache *c, const void *q, int dtype, int64_t q_row, int
                 set_error("wt_kv_attend: a captured call needs a workspace of its own (%lld bytes)", (long long)p.bytes);
                 return WT_E_CAPTURE;
             }
-            bool fresh = false;
-            if ((rc = scratch_kv(st, (size_t)p.bytes, &workspace, &fresh))) return rc;
-            if (fresh) hipLaunchKernelGGL(kv_zero_kernel, dim3(WT_KV_WORKSPACE_ZEROED / 1024), dim3(256), 0, st, (int32_t *)workspace);
+            if ((rc = scratch_kv(st, (size_t)kv_workspace(p.n_wg, 256), &workspace))) return rc;
         }
     }
     KvAttend a;

@@ -7,7 +7,9 @@
 
 #include <cmath>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -56,6 +58,11 @@ const at::Tensor &tensor(PyObject *o, const Cache *c, const char *name, int64_t 
     return t;
 }
 bool is_none(PyObject *o) { return o == Py_None; }
+
+// Nothing here has a gradient; a call that autograd would have to record is refused rather than left out of the graph.
+void no_gradient(const at::Tensor &t, const char *name) {
+    if (t.requires_grad() && at::GradMode::is_enabled()) refuse("%s requires a gradient, which the cache's calls do not have: call them under torch.no_grad()", name);
+}
 
 int dtype_of(at::ScalarType s, const Cache *c, const char *name) {   // an 8-bit cache takes and gives any of three types, another its own
     const int dt = s == at::kFloat ? WT_DTYPE_F32 : s == at::kHalf ? WT_DTYPE_F16 : s == at::kBFloat16 ? WT_DTYPE_BF16 : -1;
@@ -158,16 +165,84 @@ PyObject *setup(PyObject *, PyObject *args) {   // error class, addresses of the
     Py_RETURN_NONE;
 }
 
-// address of a wt_kv_cache (copied), one of its tensors -> handle
-PyObject *handle(PyObject *, PyObject *const *args, Py_ssize_t n) {
+// (pages, heads, slots, head_dim): values of a row side by side, 16-byte steps, no two rows in one place
+const at::Tensor &pages(PyObject *o, const char *name, int *dtype) {
+    if (!THPVariable_Check(o)) refuse("%s: not a tensor", name);
+    const at::Tensor &t = THPVariable_Unpack(o);
+    const at::ScalarType s = t.scalar_type();
+    *dtype = s == at::kFloat ? WT_DTYPE_F32 : s == at::kHalf ? WT_DTYPE_F16 : s == at::kBFloat16 ? WT_DTYPE_BF16 : s == at::kFloat8_e4m3fn ? WT_DTYPE_E4M3 : -1;
+    if (t.layout() != at::kStrided || t.dim() != 4 || *dtype < 0)
+        refuse("%s: a 4-dimensional tensor (pages, heads, slots, head_dim) of float32, float16, bfloat16 or float8_e4m3fn", name);
+    const int64_t d = t.size(3);
+    if (t.numel() == 0 || (d != 32 && d != 64 && d != 96 && d != 128 && d != 256))
+        refuse("%s: (%ld, %ld, %ld, %ld); head_dim is 32, 64, 96, 128 or 256, nothing is empty", name, (long)t.size(0), (long)t.size(1), (long)t.size(2), (long)d);
+    if (t.size(0) > INT32_MAX || t.size(1) > 65535 || t.size(2) > INT32_MAX)
+        refuse("%s: (%ld, %ld, %ld, %ld) is beyond 32-bit page and slot numbers or 65535 heads", name, (long)t.size(0), (long)t.size(1), (long)t.size(2), (long)d);
+    bool steps = t.stride(3) == 1 && ((uintptr_t)t.const_data_ptr() & 15) == 0;
+    int order[3], n = 0;   // dimensions that have a stride to speak of, the nearest rows first
+    for (int i = 0; i < 3; ++i)
+        if (t.size(i) > 1) {
+            steps = steps && t.stride(i) * t.element_size() % 16 == 0;
+            int j = n++;
+            for (; j > 0 && t.stride(order[j - 1]) > t.stride(i); --j) order[j] = order[j - 1];
+            order[j] = i;
+        }
+    if (!steps) refuse("%s: rows must be contiguous and start on 16-byte steps (strides %ld, %ld, %ld, %ld)", name, (long)t.stride(0), (long)t.stride(1), (long)t.stride(2), (long)t.stride(3));
+    int64_t extent = d;
+    for (int i = 0; i < n; ++i) {
+        if (t.stride(order[i]) < extent) refuse("%s: rows overlap (strides %ld, %ld, %ld, %ld)", name, (long)t.stride(0), (long)t.stride(1), (long)t.stride(2), (long)t.stride(3));
+        extent += t.stride(order[i]) * (t.size(order[i]) - 1);
+    }
+    return t;
+}
+
+// k, v, k_exp or None, v_exp or None, host (tensors of the host's memory are taken, for calls that are refused in the end) ->
+// (handle, error word)
+PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     try {
-        arguments(n, 2);
-        const void *p = PyLong_AsVoidPtr(args[0]);
-        if (!p || !THPVariable_Check(args[1])) refuse("handle(address, tensor)");
-        const at::Tensor &t = THPVariable_Unpack(args[1]);
-        Cache *c = new Cache{*static_cast<const wt_kv_cache *>(p), t.is_cuda() ? (int)t.get_device() : -1, t.scalar_type()};
-        return PyCapsule_New(c, CACHE, [](PyObject *o) { delete static_cast<Cache *>(PyCapsule_GetPointer(o, CACHE)); });
+        arguments(n, 5);
+        int dtype, v_dtype;
+        const at::Tensor &k = pages(args[0], "k", &dtype), &v = pages(args[1], "v", &v_dtype);
+        if (k.requires_grad() || v.requires_grad()) refuse("k, v: pages have no gradient");
+        if (k.sizes() != v.sizes() || dtype != v_dtype) refuse("k and v differ in shape or type");
+        if (k.const_data_ptr() == v.const_data_ptr()) refuse("k and v are the same memory");
+        uint8_t *e[2] = {nullptr, nullptr};
+        for (int i = 0; i < 2; ++i) {
+            const char *name = i == 0 ? "k_exp" : "v_exp";
+            if (is_none(args[2 + i]) == (dtype == WT_DTYPE_E4M3)) refuse("%s: a float8_e4m3fn cache has exponents, another has none", name);
+            if (dtype != WT_DTYPE_E4M3) continue;
+            if (!THPVariable_Check(args[2 + i])) refuse("%s: not a tensor", name);
+            const at::Tensor &x = THPVariable_Unpack(args[2 + i]);
+            if (x.scalar_type() != at::kByte || x.dim() != 3 || x.size(0) != k.size(0) || x.size(1) != k.size(1) || x.size(2) != k.size(2) ||
+                !x.is_contiguous() || ((uintptr_t)x.const_data_ptr() & 15) || x.device() != k.device())
+                refuse("%s: contiguous uint8 (%ld, %ld, %ld) beside the pages, 16-byte aligned", name, (long)k.size(0), (long)k.size(1), (long)k.size(2));
+            e[i] = static_cast<uint8_t *>(x.data_ptr());
+        }
+        if (e[0] && e[0] == e[1]) refuse("k_exp and v_exp are the same memory");
+        const int host = PyObject_IsTrue(args[4]);
+        if (host < 0) return nullptr;
+        if (!k.is_cuda() && !(host && k.is_cpu())) refuse("k must be on the GPU: the cache's kernels only run there");
+        if (k.device() != v.device()) refuse("k and v live on different devices");
+        at::Tensor error = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(k.device()));
+        const auto stride = [](const at::Tensor &t, int i) { return t.size(i) > 1 ? t.stride(i) : 0; };
+        Cache *c = new Cache{{k.data_ptr(), v.data_ptr(), e[0], e[1], stride(k, 0), stride(k, 1), stride(k, 2), stride(v, 0), stride(v, 1), stride(v, 2),
+                              (int32_t)k.size(0), (int32_t)k.size(1), (int32_t)k.size(2), (int32_t)k.size(3), dtype, 0, error.data_ptr<int32_t>()},
+                             k.is_cuda() ? (int)k.get_device() : -1,
+                             k.scalar_type()};
+        PyObject *handle = PyCapsule_New(c, CACHE, [](PyObject *o) { delete static_cast<Cache *>(PyCapsule_GetPointer(o, CACHE)); });
+        if (!handle) {
+            delete c;
+            return nullptr;
+        }
+        PyObject *both = PyTuple_New(2);
+        if (!both) {
+            Py_DECREF(handle);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(both, 0, handle);
+        PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(error));
+        return both;
     } catch (const Refused &) {
         return nullptr;
     }
@@ -183,6 +258,7 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const Rows r = rows_of(args[3], args[4], args[5], c);
         const at::Tensor &k = tensor(args[1], c, "k", 3), &v = tensor(args[2], c, "v", 3);
         if (k.scalar_type() != v.scalar_type()) refuse("k and v differ: %s, %s", c10::toString(k.scalar_type()), c10::toString(v.scalar_type()));
+        no_gradient(k, "k"), no_gradient(v, "v");
         const int dt = dtype_of(k.scalar_type(), c, "k, v");
         const Strided ks = strided(k, c, "k", r.n, c->desc.n_heads, true), vs = strided(v, c, "v", r.n, c->desc.n_heads, true);
         if (r.n > 0) {
@@ -217,6 +293,7 @@ PyObject *gather(PyObject *, PyObject *const *args, Py_ssize_t n) {
             if (k.scalar_type() != v.scalar_type() || (!is_none(args[4]) && k.scalar_type() != type))
                 refuse("out: %s and %s", c10::toString(k.scalar_type()), c10::toString(v.scalar_type()));
             type = k.scalar_type();
+            no_gradient(k, "out[0]"), no_gradient(v, "out[1]");
             strided(k, c, "out[0]", r.n, c->desc.n_heads, true), strided(v, c, "out[1]", r.n, c->desc.n_heads, true);
             if (!k.is_contiguous() || !v.is_contiguous()) refuse("out: not contiguous");
             const char *kp = static_cast<const char *>(k.const_data_ptr()), *vp = static_cast<const char *>(v.const_data_ptr());
@@ -292,6 +369,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const at::Tensor &q = tensor(args[1], c, "q", 3);
         const int64_t heads = q.size(1);
         if (heads < 1 || heads % c->desc.n_heads || heads > INT32_MAX) refuse("q: %ld query heads over %d key heads", (long)heads, c->desc.n_heads);
+        no_gradient(q, "q");
         const int dt = dtype_of(q.scalar_type(), c, "q");
         const Strided qs = strided(q, c, "q", t.n, heads, false);
         const int32_t *lengths = int32s(args[3], c, "lengths", t.n);
@@ -305,6 +383,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
         at::Tensor out, lse, ws;
         if (!is_none(args[5])) {
             out = tensor(args[5], c, "out", 3);
+            no_gradient(out, "out");
             if (out.scalar_type() != q.scalar_type()) refuse("out: %s, not %s", c10::toString(out.scalar_type()), c10::toString(q.scalar_type()));
         }
         if (!is_none(args[7])) {
@@ -361,7 +440,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 #define WT_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL
-PyMethodDef METHODS[] = {{"setup", setup, METH_VARARGS, nullptr},           {"handle", WT_FAST(handle), nullptr},
+PyMethodDef METHODS[] = {{"setup", setup, METH_VARARGS, nullptr},           {"make", WT_FAST(make), nullptr},
                          {"append", WT_FAST(append), nullptr},              {"gather", WT_FAST(gather), nullptr},
                          {"attend", WT_FAST(attend), nullptr},              {"workspace", WT_FAST(workspace), nullptr},
                          {nullptr, nullptr, 0, nullptr}};

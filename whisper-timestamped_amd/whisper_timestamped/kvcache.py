@@ -26,8 +26,6 @@ import torch
 from . import _lib
 from ._lib import WtError
 
-_DTYPES = {torch.float32: _lib.WT_DTYPE_F32, torch.float16: _lib.WT_DTYPE_F16, torch.bfloat16: _lib.WT_DTYPE_BF16}
-_PAGE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.WT_DTYPE_E4M3}
 HEAD_DIMS = (32, 64, 96, 128, 256)
 
 
@@ -44,62 +42,16 @@ def _calls():
     return _kvcalls
 
 
-def _overlaps(t):
-    """May two elements of t share a place?  (A dimension of size one has no stride to speak of.)"""
-    extent = 1
-    for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
-        if stride < extent:
-            return True
-        extent += stride * (size - 1)
-    return False
-
-
-def _check_pages(t, name):
-    """(pages, heads, slots, head_dim), values of a row side by side, 16-byte steps, no two elements in one place."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype not in _PAGE_DTYPES:
-        raise WtError(f"{name}: a 4-dimensional tensor (pages, heads, slots, head_dim) of float32, float16, bfloat16 or float8_e4m3fn")
-    if min(t.shape) < 1 or t.shape[3] not in HEAD_DIMS:
-        raise WtError(f"{name}: shape {tuple(t.shape)}; head_dim is one of {HEAD_DIMS}, nothing is empty")
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(t.stride(i) * t.element_size() % 16 for i in range(3) if t.shape[i] > 1):
-        raise WtError(f"{name}: rows must be contiguous and start on 16-byte steps (strides {t.stride()})")
-    if _overlaps(t):
-        raise WtError(f"{name}: rows overlap (strides {t.stride()})")
-
-
 class PagedKVCache:
     """Over tensors the caller owns: ``k``, ``v`` (pages, heads, slots, head_dim), in float32, float16 or bfloat16, or in
     float8_e4m3fn with ``k_exp``, ``v_exp`` (pages, heads, slots) uint8: value = code * 2 ** (exp - 127)."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_exp: torch.Tensor | None = None, v_exp: torch.Tensor | None = None):
-        _check_pages(k, "k")
-        _check_pages(v, "v")
-        if k.shape != v.shape or k.dtype != v.dtype:
-            raise WtError(f"k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
-        if k.data_ptr() == v.data_ptr():
-            raise WtError("k and v are the same memory")
-        quantised = k.dtype == torch.float8_e4m3fn
-        for name, e in (("k_exp", k_exp), ("v_exp", v_exp)):
-            if quantised != (e is not None):
-                raise WtError(f"{name}: a float8_e4m3fn cache has exponents, another has none")
-            if quantised and (e.shape != k.shape[:3] or e.dtype != torch.uint8 or not e.is_contiguous() or e.data_ptr() % 16):
-                raise WtError(f"{name}: contiguous uint8 of shape {tuple(k.shape[:3])}, 16-byte aligned")
-        if quantised and k_exp.data_ptr() == v_exp.data_ptr():
-            raise WtError("k_exp and v_exp are the same memory")
-        if k.shape[0] > 2 ** 31 - 1 or k.shape[1] > 65535 or k.shape[2] > 2 ** 31 - 1:
-            raise WtError(f"k: shape {tuple(k.shape)} is beyond 32-bit page and slot numbers or 65535 heads")
-        _lib._need_cuda(k, "k")
-        _lib.same_device(k, v, k_exp, v_exp)
+        self._calls = _calls()
+        self._handle, self.error = self._calls.make(k, v, k_exp, v_exp, False)
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
         self.device, self.dtype = k.device, k.dtype
         self.n_pages, self.n_heads, self.page_size, self.head_dim = k.shape
-        self.error = torch.zeros(1, dtype=torch.int32, device=self.device)
-        def strides(t):    # (a dimension of size one has no stride to speak of)
-            return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
-
-        desc = _lib.KvCache(k.data_ptr(), v.data_ptr(), _lib._ptr(k_exp) or None, _lib._ptr(v_exp) or None, *strides(k), *strides(v),
-                            self.n_pages, self.n_heads, self.page_size, self.head_dim, _PAGE_DTYPES[k.dtype], 0, self.error.data_ptr())
-        self._calls = _calls()
-        self._handle = self._calls.handle(ctypes.addressof(desc), k)
 
     @classmethod
     def allocate(cls, n_pages: int, n_heads: int, head_dim: int, page_size: int = 64, dtype=torch.float16, device="cuda"):
