@@ -335,11 +335,15 @@ static int kv_plan(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_wi
     const int64_t pairs = (int64_t)n_seqs * c->n_heads * ((group + 15) / 16);
     const int64_t key_bytes = 2ll * c->head_dim * (c->dtype == WT_DTYPE_F32 ? 4 : c->dtype == WT_DTYPE_E4M3 ? 1 : 2);   // and its value's
     p->n_wg = n < WT_KV_WORKSPACE_ZEROED / 16 ? n : WT_KV_WORKSPACE_ZEROED / 16;   // (four counters each)
-    p->min_share = 4;
+    // A share is at least two units (blocks of KV_WAVES waves: 16 to 64 KB), one of 128 KB: 8 pairs of 512 KB, 1 / 2 / 4 units: f16, 64
+    // values 13.6 / 11.9 / 13.3 us, bf16, 128 values 13.7 / 13.7 / 17.1, 256 values 16.7 / 20.5 / 25.4.  A segment of its own costs about two
+    // (16 sequences up to 32768, without / 2 / 4 / 8: 107 / 64 / 65 / 68 us).
+    p->min_share = key_bytes * KV_WAVES * (c->dtype == WT_DTYPE_F32 ? 16 : 32) >= 128 * 1024 ? 1 : 2;
     p->seg_cost = 2;
-    // One workgroup streams 512 KB of keys and values in about the time that splitting them costs (measured, 8 to 640 pairs in
-    // four types: 256 KB 9.6 us against 13.3, 512 KB 13.9 against 14.7, 1 MB 27.6 against 16.2).
-    p->direct = (int64_t)table_width * c->page_size * key_bytes <= 512 * 1024 && pairs <= KV_MAX_GRID;
+    // One workgroup streams keys and values at some 48 GB/s whatever its waves (four 8.8 us, eight 9.7, sixteen 11.5 over 250 KB), and
+    // splitting them costs about 6 us.  Direct / shares, us: 8 and 32 pairs (f16, 64 values) of 256 KB 8.8 / 10.3 and 9.7 / 11.1, of 384 KB
+    // 11.5 / 11.4 and 13.5 / 12.1, of 512 KB 14.2 / 11.8 and 16.7 / 13.1; 128 pairs of 512 KB 19.0 / 18.7; 256 of 512 KB 22.8 / 24.6.
+    p->direct = (int64_t)table_width * c->page_size * key_bytes <= (pairs <= n / 4 ? 384 : 512) * 1024 && pairs <= KV_MAX_GRID;
     // Where the pairs fill the card by themselves, workgroups of two waves let more of them run at once.  Four / two waves, us:
     // f16, 64 values, 256 pairs of 1..448 keys 6.6 / 7.2, 512 9.4 / 8.7, 1536 17.6 / 15.0, 5120 44.4 / 36.1; bf16, 128 values, 768 of 448
     // 35.4 / 31.7; f32, 768 of 10..1000 34.8 / 38.6, 1536 of 1..448 27.5 / 24.1; 8 bits, 1536 of 10..1000 18.2 / 21.3, 5120 of 1..448 26.0 /
