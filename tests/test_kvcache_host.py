@@ -245,3 +245,16 @@ def test_attend_wrong_python_types():
         host_cache().attend_workspace("x", TABLE)
     with pytest.raises(WtError, match="0 query heads"):
         host_cache().attend_workspace(0, TABLE)
+
+
+def test_the_cache_keeps_its_memory():
+    """What a call's addresses point into is held by the cache itself, whatever becomes of the tensors that named it."""
+    from whisper_timestamped import kvcache
+    k, v = pages(4, 2, 16, 64, dtype=E4M3), pages(4, 2, 16, 64, dtype=E4M3)
+    e = [pages(4, 2, 16, dtype=torch.uint8) for _ in range(2)]
+    uses = lambda: [torch._C._storage_Use_Count(t.untyped_storage()._cdata) for t in (k, v, *e)]
+    before = uses()
+    handle, error = kvcache._calls().make(k, v, *e, True)
+    assert uses() == [n + 1 for n in before]
+    del handle
+    assert uses() == before

@@ -30,6 +30,7 @@ struct Cache {
     wt_kv_cache desc;
     int device;   // -1: host memory, whose every call is refused
     at::ScalarType type;
+    at::Storage kept[5];   // what desc points into lives as long as it
 };
 constexpr const char *CACHE = "wt_kv_cache";
 
@@ -208,6 +209,7 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
         if (k.sizes() != v.sizes() || dtype != v_dtype) refuse("k and v differ in shape or type");
         if (k.const_data_ptr() == v.const_data_ptr()) refuse("k and v are the same memory");
         uint8_t *e[2] = {nullptr, nullptr};
+        at::Storage es[2];
         for (int i = 0; i < 2; ++i) {
             const char *name = i == 0 ? "k_exp" : "v_exp";
             if (is_none(args[2 + i]) == (dtype == WT_DTYPE_E4M3)) refuse("%s: a float8_e4m3fn cache has exponents, another has none", name);
@@ -218,6 +220,7 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
                 !x.is_contiguous() || ((uintptr_t)x.const_data_ptr() & 15) || x.device() != k.device())
                 refuse("%s: contiguous uint8 (%ld, %ld, %ld) beside the pages, 16-byte aligned", name, (long)k.size(0), (long)k.size(1), (long)k.size(2));
             e[i] = static_cast<uint8_t *>(x.data_ptr());
+            es[i] = x.storage();
         }
         if (e[0] && e[0] == e[1]) refuse("k_exp and v_exp are the same memory");
         const int host = PyObject_IsTrue(args[4]);
@@ -229,7 +232,8 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
         Cache *c = new Cache{{k.data_ptr(), v.data_ptr(), e[0], e[1], stride(k, 0), stride(k, 1), stride(k, 2), stride(v, 0), stride(v, 1), stride(v, 2),
                               (int32_t)k.size(0), (int32_t)k.size(1), (int32_t)k.size(2), (int32_t)k.size(3), dtype, 0, error.data_ptr<int32_t>()},
                              k.is_cuda() ? (int)k.get_device() : -1,
-                             k.scalar_type()};
+                             k.scalar_type(),
+                             {k.storage(), v.storage(), es[0], es[1], error.storage()}};
         PyObject *handle = PyCapsule_New(c, CACHE, [](PyObject *o) { delete static_cast<Cache *>(PyCapsule_GetPointer(o, CACHE)); });
         if (!handle) {
             delete c;
