@@ -258,3 +258,27 @@ def test_the_cache_keeps_its_memory():
     assert uses() == [n + 1 for n in before]
     del handle
     assert uses() == before
+
+
+def test_paged_decoder_leaves_shadowed_modules_alone():
+    """A backend whose attention, or whose cache hooks, somebody else has replaced on the instance keeps its own cache."""
+    import types
+    from whisper_timestamped.paged_decoder import supported
+
+    class Attn:
+        query = key = value = out = qkv_attention = forward = None
+
+    class Model:
+        dims = types.SimpleNamespace(n_text_state=128, n_text_head=2)
+        install_kv_cache_hooks = None
+
+        def __init__(self):
+            self.decoder = types.SimpleNamespace(blocks=[types.SimpleNamespace(attn=Attn()) for _ in range(2)])
+
+    assert supported(Model(), torch.float16)
+    m = Model()
+    m.decoder.blocks[1].attn.forward = lambda x: x
+    assert not supported(m, torch.float16)
+    m = Model()
+    m.install_kv_cache_hooks = lambda cache=None: None
+    assert not supported(m, torch.float16)

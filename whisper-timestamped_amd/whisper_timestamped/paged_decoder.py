@@ -23,6 +23,7 @@ PAGE = 32
 def supported(model, dtype) -> bool:
     dims = model.dims
     return dims.n_text_state // dims.n_text_head in HEAD_DIMS and dtype in (torch.float16, torch.float32, torch.bfloat16) and \
+        not any("forward" in vars(b.attn) for b in model.decoder.blocks) and "install_kv_cache_hooks" not in vars(model) and \
         all(hasattr(b.attn, m) for b in model.decoder.blocks for m in ("query", "key", "value", "out", "qkv_attention"))
 
 
