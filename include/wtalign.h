@@ -17,8 +17,8 @@
  *  - Return value: 0 on success; <0 on error (WT_E_*), with a message
  *    retrievable through wt_last_error() (thread-local).  Nothing throws.
  *  - The library keeps lazily-allocated device scratch arenas per (device,
- *    stream): per-unit reduction words, the banded mel filterbank, and the DTW's
- *    direction bit planes (T*F/4 bytes per unit of the largest batch seen);
+ *    stream): per-unit reduction words, the banded mel filterbank, wt_kv_attend's
+ *    workspace (17 MB with 256 compute units), and the DTW's direction bit planes (T*F/4 bytes per unit of the largest batch seen);
  *    wt_shutdown() frees them.  Growing an arena is a hipMalloc: warm a stream
  *    up once before capturing calls on it into a HIP graph.
  */
@@ -33,7 +33,7 @@ extern "C" {
 
 #define WT_ABI_VERSION 5 /* 2: + wt_qk_rows_batch, wt_logprob_gather_rows, wt_dtw_batch_pattern; 3: + wt_align_batch_v3;
                             4: + wt_release_stream, wt_qk_rows_streams, wt_logmel_pad_batch; only the WT_API entries are exported (the library is built with
-                               -fvisibility=hidden); 5: + wt_logprob_digest_streams */
+                               -fvisibility=hidden); 5: + wt_logprob_digest_streams; within it: + wt_kv_append, wt_kv_gather, wt_kv_attend, wt_kv_attend_workspace */
 
 /* The exported surface: exactly the functions marked WT_API below (tests/test_host_cpu.py holds `nm -D` to it). */
 #define WT_API __attribute__((visibility("default")))
@@ -348,7 +348,8 @@ WT_API int wt_kv_gather(const wt_kv_cache *cache, void *k, void *v, int dtype, i
  *     w_t = scale * q . k_t,   out = sum_t exp(w_t - max w) v_t / sum_t exp(w_t - max w),   lse = log sum_t exp(w_t)
  * Products are summed, and maximum, sum and result held, in 32 bits; out is rounded once.  lengths[s] = 0: out = 0, lse =
  * -inf.  What pages hold behind the last position takes no part, NaN and infinities included; an infinity among the values
- * that do take part leaves its element infinite or NaN.
+ * that do take part leaves its element infinite or NaN.  Sums of values run up to exp(11) * sum |v_t| before they are divided: where
+ * that is beyond 2^128 the result is not finite, and of values below 2^-100 bits are lost.
  *   q, out : device, dtype F32 / F16 / BF16 (the cache's own; any of them over an E4M3 cache), head_dim values in a row;
  *            out may be q.  Rows beyond n_seqs are not touched
  *   lse    : optional device fp32 [n_seqs][n_q_heads]
@@ -360,7 +361,8 @@ WT_API int wt_kv_attend(const wt_kv_cache *cache, const void *q, int dtype, int6
                         const int32_t *lengths, void *out, int64_t out_row_stride, int64_t out_head_stride, float *lse,
                         void *workspace, int64_t workspace_bytes, void *stream);
 
-/* Bytes of workspace that wt_kv_attend needs on the current device for this cache and these counts (< 0: error). */
+/* Bytes of workspace that wt_kv_attend needs on the current device for this cache and these counts, or fewer sequences or
+ * pages (< 0: error). */
 WT_API int64_t wt_kv_attend_workspace(const wt_kv_cache *cache, int n_seqs, int n_q_heads, int table_width);
 
 #ifdef __cplusplus

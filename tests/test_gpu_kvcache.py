@@ -170,6 +170,18 @@ def test_attend_workspace():
             cache.attend(q, table, lens, workspace=bad)
 
 
+def test_attend_workspace_for_fewer_sequences():
+    """A workspace for a table's shape does for its first sequences too, also where only those are split."""
+    cache, table, _, _, _ = make([1792] * 16, 8, 64, 16, F16, seed=6)
+    lens = torch.full((16,), 1792, dtype=torch.int32, device=DEV)
+    ws = cache.attend_workspace(8, table)
+    assert ws is not None
+    q = queries(16, 8, 64, F16, 1).to(DEV)
+    for n in (16, 3, 1):
+        assert torch.equal(cache.attend(q[:n], table[:n], lens[:n], workspace=ws), cache.attend(q[:n], table[:n], lens[:n]))
+    assert bool((ws[:16384] == 0).all())
+
+
 @pytest.mark.parametrize("q_dtype,dtype", PAIRS)
 @pytest.mark.parametrize("scale,q_gain", [(1.0, 4.0), (-0.5, 1.0), (0.0, 1.0), (1e-3, 1.0)])
 def test_attend_scales(q_dtype, dtype, scale, q_gain):
