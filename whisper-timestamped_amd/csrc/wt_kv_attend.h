@@ -50,7 +50,9 @@ struct KvFrag {
     uint2 ke, ve;                                                                    // 8-bit pages: exponents of the lane group's 8 keys
 };
 
-template <int N>   // N bytes from a place aligned to as many of them as a power of two allows (16 at most)
+// N bytes from a place aligned to as many of them as a power of two allows (16 at most).  Non-temporal: keys and values are
+// read once; with it long calls stream at 6.57 instead of 5.67 TB/s (bf16, 128 values), 7.41 instead of 6.32 (f16, 64).
+template <int N>
 __device__ __forceinline__ void kv_fetch(uint32_t *dst, const char *src) {
     if constexpr (N == 2) dst[0] = *reinterpret_cast<const uint16_t *>(src);
     else if constexpr (N == 6) {
@@ -307,7 +309,7 @@ struct KvWave {
 #pragma unroll
                 for (int i = 0; i < EV; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[j][i]), p[j], o[i], 0, 0, 0);
         } else {
-            // a weight is the sum of two 16-bit numbers: with one alone the result is off by up to 2^-9 (bf16) where few keys
+            // a weight is the sum of two 16-bit numbers: with one alone the result is off by up to 2^-8 (bf16) where few keys
             // share the weight; with both by less than 2^-16
             // values arrive as rows (key j: EV neighbouring columns a lane) and are needed as columns: pairs of rows are
             // interleaved by byte permutes
@@ -426,7 +428,7 @@ __device__ __forceinline__ int kv_length(const KvAttend &a, int raw, bool *wrong
     *wrong = raw < 0 || raw > kv_capacity(a);
     return *wrong ? 0 : raw;
 }
-__device__ __forceinline__ uint32_t kv_div(uint64_t x, uint64_t y) {   // where the quotient fits 32 bits; the wave's operands
+__device__ __forceinline__ uint32_t kv_div(uint64_t x, uint64_t y) {   // where the quotient fits 32 bits (a share that does not is hours of work); the wave's operands
     return ((x | y) >> 32) == 0 ? (uint32_t)x / (uint32_t)y : (uint32_t)(x / y);
 }
 
@@ -636,7 +638,9 @@ __device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, in
     }
 }
 
-// Short tables: one workgroup per (sequence, key head, query tile).
+// Short tables: one workgroup per (sequence, key head, query tile).  One head is bound by what a compute unit streams and by the
+// chain length -> table -> keys -> joining waves (447 keys of 8 heads, f16, 64 values: 6.3 us), many by memory (32 sequences of 1500, 20
+// heads: 45 us, 5.4 TB/s).
 template <typename CT, typename T, int HD, int PG, int NW>
 __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_direct_kernel(const KvAttend a) {
     extern __shared__ __attribute__((aligned(16))) float kv_lds[];
@@ -645,6 +649,9 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_direct_k
     kv_segment<true, CT, T, HD, PG, NW>(w, a, kv_lds, blockIdx.x / pairs, blockIdx.x % pairs, 0, false, 0, 0, -1);
 }
 
+// Longer ones: one workgroup a compute unit, equal shares.  Bound by memory; 131071 positions of 8 heads, bf16, 128 values: 90.5 us (5.9
+// TB/s), 16 sequences of 17 ... 32768: 62.5 us (5.5), 4 of 50001 ... 65537 in 8 bits: 82 us (5.8).  Two workgroups a compute unit
+// progress unevenly: their ends lay between 55 and 106 us where one's lay between 76 and 99.
 template <typename CT, typename T, int HD, int PG, int NW>
 __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_kernel(const KvAttend a) {
     extern __shared__ __attribute__((aligned(16))) float kv_lds[];

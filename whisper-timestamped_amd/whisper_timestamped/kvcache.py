@@ -66,13 +66,13 @@ class PagedKVCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, sequences: torch.Tensor | None = None):
         """Writes rows ``k[r]``, ``v[r]`` (heads, head_dim; any row and head strides of whole 16 bytes) at ``positions[r]``
         of sequence ``sequences[r]`` (None: of sequence r).  A negative position marks a padded row: not written.  No
-        two rows of a call may name the same place."""
+        two rows of a call may name the same place, and ``k`` and ``v`` are not the cache's own memory."""
         self._calls.append(self._handle, k, v, table, positions, sequences)
 
     def gather(self, table: torch.Tensor, positions: torch.Tensor, sequences: torch.Tensor | None = None, dtype=None, out=None):
         """-> (k, v), each (rows, heads, head_dim): the rows at ``positions[r]`` of sequence ``sequences[r]``, in the cache's
         type, or from an 8-bit cache in ``dtype`` (default float32).  A negative position reads as zeros.  ``out``: two
-        contiguous tensors to write instead of new ones."""
+        contiguous tensors to write instead of new ones (not the cache's own memory)."""
         return self._calls.gather(self._handle, table, positions, sequences, dtype, out)
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, scale: float | None = None,
