@@ -47,7 +47,7 @@ struct KvFrag {
     static constexpr int VD = (EV * (int)sizeof(CT) + 3) / 4;                        // dwords of a key's values
     uint32_t k[K::NT][STEPS][KD];
     uint32_t v[K::GK][VD];
-    uint2 ke, ve;                                                                    // 8-bit pages: exponents of the lane group's 8 keys
+    uint2 ke, ve;   // 8-bit pages: exponents of the lane group's 8 keys (keys by themselves, PG 1: in .x that of key lane % 32)
 };
 
 // N bytes from a place aligned to as many of them as a power of two allows (16 at most).  Non-temporal: keys and values are
@@ -84,7 +84,7 @@ __device__ __forceinline__ void kv_fetch(uint32_t *dst, const char *src) {
 template <int PG, int NT, int GK>
 struct KvSpot {
     int64_t k[PG == 1 ? NT : 1], v[PG == 1 ? GK : 1];
-    int64_t e[PG == 1 ? GK : 1];
+    int64_t e[1];
 };
 
 template <typename CT, typename T, int HD, int PG, int NW>
@@ -153,14 +153,11 @@ struct KvWave {
             const int page = checked(id.k, &bad);
             const int slot = p - (int)(page_of(a.c.div, (uint32_t)p) * a.c.div.d);
             const int64_t kk = (page * a.k.page + h * a.k.head + slot * a.k.slot) * ITEM, vv = (page * a.v.page + h * a.v.head + slot * a.v.slot) * ITEM;
-            const int64_t ee = ((int64_t)page * a.c.n_heads + h) * a.c.page_size + slot;
+            s.e[0] = ((int64_t)page * a.c.n_heads + h) * a.c.page_size + slot;
 #pragma unroll
             for (int t = 0; t < K::NT; ++t) s.k[t] = shfl64(kk, kkey(t)) + kv_d<CT, HD>(0, g) * ITEM;
 #pragma unroll
-            for (int j = 0; j < K::GK; ++j) {
-                s.v[j] = shfl64(vv, g * K::GK + j) + n * EV * ITEM;
-                if constexpr (K::E4M3) s.e[j] = shfl64(ee, g * K::GK + j);
-            }
+            for (int j = 0; j < K::GK; ++j) s.v[j] = shfl64(vv, g * K::GK + j) + n * EV * ITEM;
         }
     }
     static __device__ __forceinline__ int64_t shfl64(int64_t v, int src) {
@@ -200,13 +197,7 @@ struct KvWave {
         }
         if constexpr (K::E4M3) {
             if constexpr (PG == 1) {
-                uint32_t w[2][2] = {{0, 0}, {0, 0}};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    w[0][j / 4] |= (uint32_t)a.k.e[s.e[j]] << (j % 4 * 8);
-                    w[1][j / 4] |= (uint32_t)a.v.e[s.e[j]] << (j % 4 * 8);
-                }
-                f.ke = {w[0][0], w[0][1]}, f.ve = {w[1][0], w[1][1]};
+                f.ke.x = a.k.e[s.e[0]], f.ve.x = a.v.e[s.e[0]];
             } else {
                 const int64_t e = s.e[0] + (PG == 32 ? g * 8 : 0);
                 f.ke = *reinterpret_cast<const uint2 *>(a.k.e + e), f.ve = *reinterpret_cast<const uint2 *>(a.v.e + e);
@@ -262,9 +253,16 @@ struct KvWave {
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[t * 4 + r] = s[r];
         }
+        // PG 1: exponents of key and value, each from the lane that has them (16 sequences of 4000 ... 12000 positions, 8 heads of 128, pages
+        // of 100: 56 us; 75 with a load of a byte for every key of the lane group)
+        uint32_t both[PG == 1 && K::E4M3 ? 8 : 1];
         if constexpr (K::E4M3) {
+            if constexpr (PG == 1) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= exp_of((j < 4 ? f.ke.x : f.ke.y) >> (j % 4 * 8) & 255u);
+                for (int j = 0; j < 8; ++j) both[j] = (uint32_t)__shfl((int)(f.ke.x | f.ve.x << 8), g * 8 + j, 64);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= exp_of((PG == 1 ? both[PG == 1 ? j : 0] : (j < 4 ? f.ke.x : f.ke.y) >> (j % 4 * 8)) & 255u);
         }
 #pragma unroll
         for (int j = 0; j < GK; ++j) x[j] *= a.scale;
@@ -299,7 +297,7 @@ struct KvWave {
         if constexpr (K::E4M3) {   // the value's power of two goes into its weight
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float e = exp_of((j < 4 ? f.ve.x : f.ve.y) >> (j % 4 * 8) & 255u);
+                const float e = exp_of((PG == 1 ? both[PG == 1 ? j : 0] >> 8 : (j < 4 ? f.ve.x : f.ve.y) >> (j % 4 * 8)) & 255u);
                 p[j] *= off >> j & 1 ? 0.f : e;
             }
         }
