@@ -32,6 +32,7 @@ CASES = {
     "split_f16": (torch.float16, torch.float16, 128, 64, 1, 3, [5000, 1, 2999]),
     "split_e4m3": (E4M3, torch.bfloat16, 128, 16, 1, 20, [4096, 4095]),
     "split_f32": (torch.float32, torch.float32, 64, 50, 1, 16, [3000, 1500]),
+    "split_bf16_48_queries": (torch.bfloat16, torch.bfloat16, 128, 24, 1, 48, [2500, 0, 3001]),
 }
 _BITS = {torch.bfloat16: torch.int16, E4M3: torch.uint8}
 

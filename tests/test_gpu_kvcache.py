@@ -114,6 +114,15 @@ def test_attend_groups(group, heads, q_dtype, dtype):
     check_attend([77, 5, 0, 1, 260], group, heads, 128, 32, q_dtype, dtype, seed=group)
 
 
+@pytest.mark.parametrize("group,page,width,lengths", [(18, 16, 32, [70, 0, 1, 33]), (32, 64, 64, [257, 31]), (33, 32, 96, [64, 5, 0]), (49, 24, 128, [1, 129]),
+                                                      (31, 10, 128, [90, 300]), (64, 3, 64, [40]), (24, 64, 128, [40001]), (32, 100, 128, [9000, 0, 1, 3001]),
+                                                      (17, 16, 96, [12000, 700]), (48, 32, 32, [30001]), (24, 16, 256, [5000, 17])])
+@pytest.mark.parametrize("q_dtype,dtype", PAIRS)
+def test_attend_wide_groups(group, page, width, lengths, q_dtype, dtype):
+    """More than 16 query heads a key head: two tiles of them at a time, whole and split, with joins in groups."""
+    check_attend(lengths, group, 1, width, page, q_dtype, dtype, seed=group)
+
+
 @pytest.mark.parametrize("layout", ["page_slot_head", "side_by_side"])
 @pytest.mark.parametrize("q_dtype,dtype", PAIRS)
 def test_attend_layouts(layout, q_dtype, dtype):

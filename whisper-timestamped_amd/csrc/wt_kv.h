@@ -98,7 +98,9 @@ static_assert(sizeof(Pack<float, 6>) == 24 && sizeof(Pack<uint16_t, 6>) == 12 &&
 
 constexpr int KV_WAVES = 4;   // waves of a workgroup of the attention kernel
 
-constexpr int kv_slot(int head_dim) { return 64 + 16 * head_dim; }   // floats of a partial result
+constexpr int KV_WIDE_HD = 128;   // widest heads whose queries may be taken 32 at a time (beyond, registers run out)
+
+constexpr int kv_slot(int head_dim, int q_wide) { return q_wide * (64 + 16 * head_dim); }   // floats of a partial result
 
 // arguments of one attention call, as its kernels take them (wt_kv_attend.h)
 struct KvAttend {
@@ -107,7 +109,8 @@ struct KvAttend {
     KvTable t;
     const void *q;
     int64_t q_row, q_head;
-    int n_q_heads, group, q_tiles;   // query heads a key head, tiles of 16 of them
+    int n_q_heads, group;            // query heads, those of a key head
+    int q_wide, q_tiles;             // ... are taken 16 * q_wide at a time, in q_tiles tiles
     float scale;
     const int32_t *lengths;
     void *out;
@@ -119,7 +122,7 @@ struct KvAttend {
     int waves;                       // of a workgroup: KV_WAVES, or 2
     int n_wg, min_share, seg_cost;
     int32_t *counters;               // 4 * n_wg, zero between calls
-    float *partials;                 // 2 * n_wg slots: maxima and sums of 16 queries, the same of a joined group, sums of values
+    float *partials;                 // 2 * n_wg slots: a tile's maxima and sums, the same of a joined group, sums of values
 };
 
 }  // namespace wt

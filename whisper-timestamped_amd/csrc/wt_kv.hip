@@ -314,12 +314,16 @@ int kv_clear(void *workspace, hipStream_t st) {
     WT_HIP(hipGetLastError());
     return WT_OK;
 }
-static int64_t kv_workspace(int n_wg, int head_dim) { return WT_KV_WORKSPACE_ZEROED + (int64_t)n_wg * 2 * kv_slot(head_dim) * 4; }
+static int64_t kv_workspace(int n_wg, int head_dim, int q_wide) { return WT_KV_WORKSPACE_ZEROED + (int64_t)n_wg * 2 * kv_slot(head_dim, q_wide) * 4; }
+static int64_t kv_most_workspace(int n_wg) {   // of any call
+    const int64_t narrow = kv_workspace(n_wg, 256, 1), wide = kv_workspace(n_wg, KV_WIDE_HD, 2);
+    return narrow > wide ? narrow : wide;
+}
 
 constexpr int64_t KV_MAX_GRID = 1 << 23;   // workgroups of one launch: a grid has less than 2^32 threads
 
 struct KvPlan {
-    int direct, waves, n_wg, min_share, seg_cost;
+    int q_wide, q_tiles, direct, waves, n_wg, min_share, seg_cost;
     unsigned grid;
     int64_t bytes;
 };
@@ -334,7 +338,7 @@ static int kv_plan(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_wi
         if (dev < 16) cus[dev] = n;
     }
     const int group = n_q_heads / c->n_heads;
-    const int64_t pairs = (int64_t)n_seqs * c->n_heads * ((group + 15) / 16);
+    const int64_t heads = (int64_t)n_seqs * c->n_heads, narrow = heads * ((group + 15) / 16);
     const int64_t key_bytes = 2ll * c->head_dim * (c->dtype == WT_DTYPE_F32 ? 4 : c->dtype == WT_DTYPE_E4M3 ? 1 : 2);   // and its value's
     p->n_wg = n < WT_KV_WORKSPACE_ZEROED / 16 ? n : WT_KV_WORKSPACE_ZEROED / 16;   // (four counters each)
     // A share is at least two units (blocks of KV_WAVES waves: 16 to 64 KB), one of 128 KB: 8 pairs of 512 KB, 1 / 2 / 4 units: f16, 64
@@ -345,14 +349,28 @@ static int kv_plan(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_wi
     // One workgroup streams keys and values at some 48 GB/s whatever its waves (four 8.8 us, eight 9.7, sixteen 11.5 over 250 KB), and
     // splitting them costs about 6 us.  Direct / shares, us: 8 and 32 pairs (f16, 64 values) of 256 KB 8.8 / 10.3 and 9.7 / 11.1, of 384 KB
     // 11.5 / 11.4 and 13.5 / 12.1, of 512 KB 14.2 / 11.8 and 16.7 / 13.1; 128 pairs of 512 KB 19.0 / 18.7; 256 of 512 KB 22.8 / 24.6.
-    p->direct = (int64_t)table_width * c->page_size * key_bytes <= (pairs <= n / 4 ? 384 : 512) * 1024 && pairs <= KV_MAX_GRID;
+    const int64_t capacity = (int64_t)table_width * c->page_size * key_bytes;
+    const auto is_direct = [&](int64_t pairs) { return capacity <= (pairs <= n / 4 ? 384 : 512) * 1024 && pairs <= KV_MAX_GRID; };
+    // More than 16 query heads a key head: 32 at a time read keys and values half as often, but leave one wave a SIMD where a key is more than
+    // 64 values of 16 bits, and their partial results are twice as long.  16 / 32 at a time, us, 24 query heads a key head.  Whole tables of
+    // 448 keys, 128, 256 and 384 tiles of 16: bf16, 128 values 12.5 / 14.1, 14.5 / 14.8, 23.2 / 15.5, f32, 64 values 11.7 / 13.7, 13.1 /
+    // 14.0, 21.0 / 14.4.  5120 tiles of 32, 128, 224, 448 keys: bf16, 128 values 41 / 59, 86 / 85, 117 / 102, 188 / 137, 96 values 30 / 53, 49 /
+    // 65, 73 / 81, 125 / 106, 8 bits, 128 values 34 / 60, 50 / 71, 65 / 82, 104 / 102; f16, 64 values 21 / 21, 44 / 31, 59 / 40, 94 / 58, f32, 64
+    // values 39 / 27 ... 179 / 106, 128 values 81 / 76 ... 402 / 238.  Shares, tables of 50, 100, 300 (8 bits) or 600 MB in all: bf16, 128 values
+    // 28.7 / 33.3, 47 / 41, 195 / 115, f16, 64 values 25.2 / 25.4, 40 / 35, 100 / 62, 8 bits, 128 values 33 / 35, 48 / 49, 107 / 77.
+    const bool widen = is_direct(narrow) ? narrow > n && (c->head_dim <= 64 || c->dtype == WT_DTYPE_F32 || capacity >= 128 * 1024)
+                                         : heads * capacity >= 80 * 1024 * 1024;
+    p->q_wide = group > 16 && c->head_dim <= KV_WIDE_HD && widen ? 2 : 1;
+    p->q_tiles = (group + 16 * p->q_wide - 1) / (16 * p->q_wide);
+    const int64_t pairs = heads * p->q_tiles;
+    p->direct = is_direct(pairs);
     // Where the pairs fill the card by themselves, workgroups of two waves let more of them run at once.  Four / two waves, us:
     // f16, 64 values, 256 pairs of 1..448 keys 6.6 / 7.2, 512 9.4 / 8.7, 1536 17.6 / 15.0, 5120 44.4 / 36.1; bf16, 128 values, 768 of 448
     // 35.4 / 31.7; f32, 768 of 10..1000 34.8 / 38.6, 1536 of 1..448 27.5 / 24.1; 8 bits, 1536 of 10..1000 18.2 / 21.3, 5120 of 1..448 26.0 /
     // 23.0.  (One wave: 5120 pairs of 128 keys each 32.9 against 39.8 with two, but of 1..448 keys 44.6 against 36.1.)
-    p->waves = p->direct && pairs >= n * (c->dtype == WT_DTYPE_F32 ? 6 : c->dtype == WT_DTYPE_E4M3 ? 12 : 2) ? 2 : KV_WAVES;
+    p->waves = p->direct && p->q_wide == 1 && pairs >= n * (c->dtype == WT_DTYPE_F32 ? 6 : c->dtype == WT_DTYPE_E4M3 ? 12 : 2) ? 2 : KV_WAVES;
     p->grid = p->direct ? (unsigned)pairs : (unsigned)p->n_wg;
-    p->bytes = p->direct ? 0 : kv_workspace(p->n_wg, c->head_dim);
+    p->bytes = p->direct ? 0 : kv_workspace(p->n_wg, c->head_dim, p->q_wide);
     return WT_OK;
 }
 
@@ -409,13 +427,13 @@ int kv_attend(const wt_kv_cache *c, const void *q, int dtype, int64_t q_row, int
                 set_error("wt_kv_attend: a captured call needs a workspace of its own (%lld bytes)", (long long)p.bytes);
                 return WT_E_CAPTURE;
             }
-            if ((rc = scratch_kv(st, (size_t)kv_workspace(p.n_wg, 256), &workspace))) return rc;
+            if ((rc = scratch_kv(st, (size_t)kv_most_workspace(p.n_wg), &workspace))) return rc;
         }
     }
     KvAttend a;
     a.k = kv_k(c), a.v = kv_v(c), a.c = kv_dims(c), a.t = KvTable{table, table_stride, n_seqs, table_width};
     a.q = q, a.q_row = q_row, a.q_head = q_head;
-    a.n_q_heads = n_q_heads, a.group = n_q_heads / c->n_heads, a.q_tiles = (a.group + 15) / 16;
+    a.n_q_heads = n_q_heads, a.group = n_q_heads / c->n_heads, a.q_wide = p.q_wide, a.q_tiles = p.q_tiles;
     a.scale = scale, a.lengths = lengths, a.out = out, a.o_row = o_row, a.o_head = o_head, a.lse = lse;
     a.q_aligned = (((uintptr_t)q | (uint64_t)(q_row * item) | (uint64_t)(q_head * item)) & 15) == 0;
     a.o_aligned = (((uintptr_t)out | (uint64_t)(o_row * item) | (uint64_t)(o_head * item)) & (4 * item - 1)) == 0;

@@ -87,7 +87,8 @@ struct KvSpot {
     int64_t e[1];
 };
 
-template <typename CT, typename T, int HD, int PG, int NW>
+// A wave's share of one (sequence, key head, tile of 16 * QT queries)
+template <typename CT, typename T, int HD, int PG, int NW, int QT>
 struct KvWave {
     using K = KvKind<CT, T, HD>;
     using Frag = KvFrag<CT, T, HD>;
@@ -101,11 +102,11 @@ struct KvWave {
     bool bad = false;
     uint32_t koff, voff;  // PG 32: this lane's byte offsets inside a page
     // queries
-    u4 q[K::F32 ? 1 : K::QP][K::F32 ? 1 : STEPS];
-    f4 qf[K::F32 ? STEPS : 1];
+    u4 q[QT][K::F32 ? 1 : K::QP][K::F32 ? 1 : STEPS];
+    f4 qf[QT][K::F32 ? STEPS : 1];
     // state
-    f4 o[EV];
-    float m, l;
+    f4 o[QT][EV];
+    float m[QT], l[QT];
 
     __device__ __forceinline__ KvWave(const KvAttend &args) : a(args), lane(threadIdx.x & 63), g((threadIdx.x & 63) >> 4), n(threadIdx.x & 15) {}
 
@@ -232,26 +233,34 @@ struct KvWave {
     // weights), whose contraction slots are numbered alike.
     __device__ __forceinline__ void block(Frag &f, int p0) {
         constexpr int GK = K::GK;
-        float x[GK];
+        float x[QT][GK];
 #pragma unroll
         for (int t = 0; t < K::NT; ++t) {
-            f4 s = {0.f, 0.f, 0.f, 0.f};
+            f4 s[QT];
+#pragma unroll
+            for (int y = 0; y < QT; ++y) s[y] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
                 if constexpr (K::F32) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.k[t][st][i]), qf[st][i], s, 0, 0, 0);
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int y = 0; y < QT; ++y) s[y] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.k[t][st][i]), qf[y][st][i], s[y], 0, 0, 0);
                 } else {
                     u4 w;
                     if constexpr (K::E4M3)
                         w = u4{codes(f.k[t][st][0], false), codes(f.k[t][st][0], true), codes(f.k[t][st][1], false), codes(f.k[t][st][1], true)};
                     else w = u4{f.k[t][st][0], f.k[t][st][1], f.k[t][st][2], f.k[t][st][3]};
 #pragma unroll
-                    for (int p = K::QP - 1; p >= 0; --p) s = mma(w, q[p][st], s);
+                    for (int p = K::QP - 1; p >= 0; --p)
+#pragma unroll
+                        for (int y = 0; y < QT; ++y) s[y] = mma(w, q[y][p][st], s[y]);
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[t * 4 + r] = s[r];
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int y = 0; y < QT; ++y) x[y][t * 4 + r] = s[y][r];
         }
         // PG 1: exponents of key and value, each from the lane that has them (16 sequences of 4000 ... 12000 positions, 8 heads of 128, pages
         // of 100: 56 us; 75 with a load of a byte for every key of the lane group)
@@ -262,61 +271,76 @@ struct KvWave {
                 for (int j = 0; j < 8; ++j) both[j] = (uint32_t)__shfl((int)(f.ke.x | f.ve.x << 8), g * 8 + j, 64);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= exp_of((PG == 1 ? both[PG == 1 ? j : 0] : (j < 4 ? f.ke.x : f.ke.y) >> (j % 4 * 8)) & 255u);
+            for (int j = 0; j < 8; ++j) {
+                const float e = exp_of((PG == 1 ? both[PG == 1 ? j : 0] : (j < 4 ? f.ke.x : f.ke.y) >> (j % 4 * 8)) & 255u);
+#pragma unroll
+                for (int y = 0; y < QT; ++y) x[y][j] *= e;
+            }
         }
 #pragma unroll
-        for (int j = 0; j < GK; ++j) x[j] *= a.scale;
+        for (int y = 0; y < QT; ++y)
+#pragma unroll
+            for (int j = 0; j < GK; ++j) x[y][j] *= a.scale;
         uint32_t off = 0;   // keys of this lane group behind the end
         if (p0 + K::KB > len) {
 #pragma unroll
             for (int j = 0; j < GK; ++j)
                 if (p0 + g * GK + j >= len) {
                     off |= 1u << j;
-                    x[j] = -__builtin_inff();
+#pragma unroll
+                    for (int y = 0; y < QT; ++y) x[y][j] = -__builtin_inff();
 #pragma unroll
                     for (int i = 0; i < Frag::VD; ++i) f.v[j][i] = 0;
                 }
         }
-        float top = x[0];
+        float p[QT][GK];
 #pragma unroll
-        for (int j = 1; j < GK; ++j) top = fmaxf(top, x[j]);
-        if (__any(top > m + (K::BIAS + K::SLACK))) {   // rare once the maximum is found: the reference moves, all sums with it
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m, top - K::BIAS), c = __builtin_amdgcn_exp2f((m - mn) * KV_LOG2E);
-            m = mn;
-            l *= c;
+        for (int y = 0; y < QT; ++y) {
+            float top = x[y][0];
 #pragma unroll
-            for (int i = 0; i < EV; ++i) o[i] *= c;
+            for (int j = 1; j < GK; ++j) top = fmaxf(top, x[y][j]);
+            if (__any(top > m[y] + (K::BIAS + K::SLACK))) {   // rare once the maximum is found: the reference moves, all sums with it
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float mn = fmaxf(m[y], top - K::BIAS), c = __builtin_amdgcn_exp2f((m[y] - mn) * KV_LOG2E);
+                m[y] = mn;
+                l[y] *= c;
+#pragma unroll
+                for (int i = 0; i < EV; ++i) o[y][i] *= c;
+            }
+#pragma unroll
+            for (int j = 0; j < GK; ++j) p[y][j] = __builtin_amdgcn_exp2f((x[y][j] - m[y]) * KV_LOG2E);
+#pragma unroll
+            for (int j = 0; j < GK; ++j) l[y] += p[y][j];
         }
-        float p[GK];
-#pragma unroll
-        for (int j = 0; j < GK; ++j) p[j] = __builtin_amdgcn_exp2f((x[j] - m) * KV_LOG2E);
-#pragma unroll
-        for (int j = 0; j < GK; ++j) l += p[j];
         if constexpr (K::E4M3) {   // the value's power of two goes into its weight
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float e = exp_of((PG == 1 ? both[PG == 1 ? j : 0] >> 8 : (j < 4 ? f.ve.x : f.ve.y) >> (j % 4 * 8)) & 255u);
-                p[j] *= off >> j & 1 ? 0.f : e;
+#pragma unroll
+                for (int y = 0; y < QT; ++y) p[y][j] *= off >> j & 1 ? 0.f : e;
             }
         }
         if constexpr (K::F32) {
 #pragma unroll
             for (int j = 0; j < GK; ++j)
 #pragma unroll
-                for (int i = 0; i < EV; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[j][i]), p[j], o[i], 0, 0, 0);
+                for (int i = 0; i < EV; ++i)
+#pragma unroll
+                    for (int y = 0; y < QT; ++y) o[y][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[j][i]), p[y][j], o[y][i], 0, 0, 0);
         } else {
             // a weight is the sum of two 16-bit numbers: with one alone the result is off by up to 2^-8 (bf16) where few keys
             // share the weight; with both by less than 2^-16
             // values arrive as rows (key j: EV neighbouring columns a lane) and are needed as columns: pairs of rows are
             // interleaved by byte permutes
-            u4 hi, lo;
+            u4 hi[QT], lo[QT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                hi[i] = pack16(p[2 * i], p[2 * i + 1]);
-                lo[i] = pack16(p[2 * i] - low16(hi[i]), p[2 * i + 1] - high16(hi[i]));
-            }
+            for (int y = 0; y < QT; ++y)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    hi[y][i] = pack16(p[y][2 * i], p[y][2 * i + 1]);
+                    lo[y][i] = pack16(p[y][2 * i] - low16(hi[y][i]), p[y][2 * i + 1] - high16(hi[y][i]));
+                }
             uint32_t w[8][EV / 2];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -331,8 +355,10 @@ struct KvWave {
 #pragma unroll
                 for (int jj = 0; jj < 4; ++jj)
                     vt[jj] = __builtin_amdgcn_perm(w[2 * jj + 1][i / 2], w[2 * jj][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
-                o[i] = mma(vt, lo, o[i]);
-                o[i] = mma(vt, hi, o[i]);
+#pragma unroll
+                for (int y = 0; y < QT; ++y) o[y][i] = mma(vt, lo[y], o[y][i]);
+#pragma unroll
+                for (int y = 0; y < QT; ++y) o[y][i] = mma(vt, hi[y], o[y][i]);
             }
         }
     }
@@ -340,43 +366,49 @@ struct KvWave {
     // the queries in two steps, so that the first block's loads are on their way before the conversion waits
     static constexpr int QE = K::F32 ? 4 : 8;
     struct Raw {
-        Pack<T, QE> p[STEPS];
+        Pack<T, QE> p[QT][STEPS];
     };
     __device__ __forceinline__ void queries_load(Raw &raw, int s, int hq0, int rows) const {
-        const T *src = static_cast<const T *>(a.q) + s * a.q_row + (hq0 + min(n, rows - 1)) * a.q_head;
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-            const int d = kv_d<CT, HD>(st, g);
-            if (a.q_aligned) raw.p[st] = *reinterpret_cast<const Pack<T, QE> *>(src + d);
-            else {
+        for (int y = 0; y < QT; ++y) {
+            const T *src = static_cast<const T *>(a.q) + s * a.q_row + (hq0 + min(y * 16 + n, rows - 1)) * a.q_head;
 #pragma unroll
-                for (int i = 0; i < QE; ++i) raw.p[st].v[i] = src[d + i];
+            for (int st = 0; st < STEPS; ++st) {
+                const int d = kv_d<CT, HD>(st, g);
+                if (a.q_aligned) raw.p[y][st] = *reinterpret_cast<const Pack<T, QE> *>(src + d);
+                else {
+#pragma unroll
+                    for (int i = 0; i < QE; ++i) raw.p[y][st].v[i] = src[d + i];
+                }
             }
         }
     }
     __device__ __forceinline__ void queries_take(const Raw &raw, int rows) {   // columns without a query are zeros
-        const bool in = n < rows;
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-            if constexpr (K::F32) {
+        for (int y = 0; y < QT; ++y) {
+            const bool in = y * 16 + n < rows;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) qf[st][i] = in ? raw.p[st].v[i] : 0.f;
-            } else if constexpr (K::QP == 1) {
-                const u4 w = __builtin_bit_cast(u4, raw.p[st]);
+            for (int st = 0; st < STEPS; ++st) {
+                if constexpr (K::F32) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) q[0][st][i] = in ? w[i] : 0u;
-            } else {
-                float v[8];
+                    for (int i = 0; i < 4; ++i) qf[y][st][i] = in ? raw.p[y][st].v[i] : 0.f;
+                } else if constexpr (K::QP == 1) {
+                    const u4 w = __builtin_bit_cast(u4, raw.p[y][st]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = in ? to_f(raw.p[st].v[i]) : 0.f;
+                    for (int i = 0; i < 4; ++i) q[y][0][st][i] = in ? w[i] : 0u;
+                } else {
+                    float v[8];
 #pragma unroll
-                for (int p = 0; p < K::QP; ++p)
+                    for (int i = 0; i < 8; ++i) v[i] = in ? to_f(raw.p[y][st].v[i]) : 0.f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t w = pack16(v[2 * i], v[2 * i + 1]);
-                        q[p][st][i] = w;
-                        v[2 * i] -= low16(w), v[2 * i + 1] -= high16(w);
-                    }
+                    for (int p = 0; p < K::QP; ++p)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t w = pack16(v[2 * i], v[2 * i + 1]);
+                            q[y][p][st][i] = w;
+                            v[2 * i] -= low16(w), v[2 * i + 1] -= high16(w);
+                        }
+                }
             }
         }
     }
@@ -384,9 +416,12 @@ struct KvWave {
     // blocks b, b + NW, ... < end of this sequence and head; two sets of registers, the next block's loads always in
     // flight.  `first`: table entries of block b, loaded before the length was known (and not clamped to it).
     __device__ __forceinline__ void run(int b, int end, Ids first, const Raw &raw, int rows) {
-        m = KV_LOWEST, l = 0.f;
 #pragma unroll
-        for (int i = 0; i < EV; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int y = 0; y < QT; ++y) {
+            m[y] = KV_LOWEST, l[y] = 0.f;
+#pragma unroll
+            for (int i = 0; i < EV; ++i) o[y][i] = f4{0.f, 0.f, 0.f, 0.f};
+        }
         if (b >= end) return;
         if constexpr (PG == 32) {
             koff = (uint32_t)(kkey(0) * (uint32_t)a.k.slot + kv_d<CT, HD>(0, g)) * ITEM;
@@ -434,8 +469,9 @@ __device__ __forceinline__ uint32_t kv_div(uint64_t x, uint64_t y) {   // where 
 // loaded from there (the agent's scope in the instruction itself).  Fences of that scope around plain stores write back and
 // invalidate whole L2s: with them, 131071 positions took 246 us instead of 171.
 constexpr int KV_AGENT = 16;
+template <int HD, int QT>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t kv_partials(const KvAttend &a) {
-    return __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, a.n_wg * 2 * kv_slot(a.c.head_dim) * 4, 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, a.n_wg * 2 * kv_slot(HD, QT) * 4, 0x00020000);
 }
 __device__ __forceinline__ void kv_put(__amdgpu_buffer_rsrc_t p, int at, float v) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), p, at * 4, 0, KV_AGENT); }
 __device__ __forceinline__ void kv_put(__amdgpu_buffer_rsrc_t p, int at, f4 v) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), p, at * 4, 0, KV_AGENT); }
@@ -458,15 +494,15 @@ __device__ __forceinline__ void kv_result(const KvAttend &a, int s, int head, in
 // One workgroup's part of one (sequence, key head, query tile): blocks [b0, b1).  What the waves found is joined in LDS and
 // goes out as the result, or as a partial one (slot >= 0).  LATE: the length is not known yet (all blocks are meant then):
 // queries and first table entries are loaded beside it.
-template <bool LATE, typename CT, typename T, int HD, int PG, int NW>
-__device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW> &w, const KvAttend &a, float *lds, int s, int pair, int len, bool bad_len,
+template <bool LATE, typename CT, typename T, int HD, int PG, int NW, int QT>
+__device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW, QT> &w, const KvAttend &a, float *lds, int s, int pair, int len, bool bad_len,
                                            int b0, int b1, int slot) {
-    constexpr int EV = HD / 16, KB = KvKind<CT, T, HD>::KB;
+    constexpr int EV = HD / 16, KB = KvKind<CT, T, HD>::KB, R = 16 * QT;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = pair / a.q_tiles, qt = pair % a.q_tiles;
-    const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
+    const int hq0 = h * a.group + qt * R, rows = min(R, a.group - qt * R);
     w.row = a.t.t + s * a.t.stride;
     w.h = h;
-    typename KvWave<CT, T, HD, PG, NW>::Raw raw;
+    typename KvWave<CT, T, HD, PG, NW, QT>::Raw raw;
     const int late_len = LATE ? a.lengths[s] : 0;
     const auto first = w.ids((b0 + wave) * KB, LATE ? (int)kv_capacity(a) : max(len, 1));
     w.queries_load(raw, s, hq0, rows);
@@ -478,39 +514,43 @@ __device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW> &w, const K
     w.bad = bad_len;
     w.run(b0 + wave, b1, first, raw, rows);
     if (__any(w.bad) && w.lane == 0) kv_report(a.c.error, bad_len ? WT_KV_BAD_POSITION : WT_KV_BAD_PAGE);
-    if (__any(w.bad)) w.l = __builtin_nanf("");
-    float *lm = lds, *ll = lds + NW * 16, *lo = lds + NW * 32;
-    float l = w.l;
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (w.lane < 16) lm[wave * 16 + w.n] = w.m, ll[wave * 16 + w.n] = l;
-    if (w.n < rows) {
+    const bool bad = __any(w.bad);
+    float *lm = lds, *ll = lds + NW * R, *lo = lds + NW * 2 * R;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+    for (int y = 0; y < QT; ++y) {
+        float l = bad ? __builtin_nanf("") : w.l[y];
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        const int r = y * 16 + w.n;
+        if (w.lane < 16) lm[wave * R + r] = w.m[y], ll[wave * R + r] = l;
+        if (r < rows) {
 #pragma unroll
-            for (int i = 0; i < EV; ++i) lo[(wave * rows + w.n) * HD + (4 * w.g + r) * EV + i] = w.o[i][r];
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int i = 0; i < EV; ++i) lo[(wave * rows + r) * HD + (4 * w.g + x) * EV + i] = w.o[y][i][x];
+        }
     }
     __syncthreads();
-    const __amdgpu_buffer_rsrc_t part = kv_partials(a);
-    const int at = slot * kv_slot(HD);
+    const __amdgpu_buffer_rsrc_t part = kv_partials<HD, QT>(a);
+    const int at = slot * kv_slot(HD, QT);
     for (int e = threadIdx.x; e < rows * (HD / 4); e += NW * 64) {
         const int r = e / (HD / 4), d = e % (HD / 4) * 4;
         float mm = lm[r];
 #pragma unroll
-        for (int i = 1; i < NW; ++i) mm = fmaxf(mm, lm[i * 16 + r]);
+        for (int i = 1; i < NW; ++i) mm = fmaxf(mm, lm[i * R + r]);
         f4 acc = {0.f, 0.f, 0.f, 0.f};
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-            const float c = __builtin_amdgcn_exp2f((lm[i * 16 + r] - mm) * KV_LOG2E);
+            const float c = __builtin_amdgcn_exp2f((lm[i * R + r] - mm) * KV_LOG2E);
             const f4 x = *reinterpret_cast<const f4 *>(&lo[(i * rows + r) * HD + d]);
 #pragma unroll
             for (int y = 0; y < 4; ++y) acc[y] = fmaf(x[y], c, acc[y]);
-            sum = fmaf(ll[i * 16 + r], c, sum);
+            sum = fmaf(ll[i * R + r], c, sum);
         }
         if (slot >= 0) {
-            kv_put(part, at + 64 + e * 4, acc);
-            if (d == 0) kv_put(part, at + r, mm), kv_put(part, at + 16 + r, sum);
+            kv_put(part, at + 4 * R + e * 4, acc);
+            if (d == 0) kv_put(part, at + r, mm), kv_put(part, at + R + r, sum);
         } else {
             const bool empty = len == 0 && !bad_len;
 #pragma unroll
@@ -522,18 +562,21 @@ __device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW> &w, const K
 }
 
 // The last workgroup of a pair to arrive joins its partial results.  A thread takes four columns of a row, and where there
-// are more threads than that, every LANES-th part; KV_JOIN parts are loaded at a time, in an order that never changes.  With
-// more than two KV_GROUPs of parts the last of each group joins the group, and the last of those the groups (90 parts of 8
-// queries of 256 values: 30 us by one workgroup alone).
-constexpr int KV_JOIN = 8, KV_GROUP = 16;
+// are more threads than that, every LANES-th part; KV_JOIN parts are loaded at a time, in an order that never changes.  One workgroup
+// reads partial results at some 48 GB/s, so with more than two KV_GROUPs of parts the last of each group joins the group, and the
+// last of those the groups, and so on (90 parts of 8 queries of 256 values: 30 us by one workgroup alone; 24 queries of 128 values,
+// 8 heads of 12000 positions, groups of 16 / 12 / 8 / 6: 43.6 / 38.1 / 33.3 / 33.2 us, of 40000 114.9 / 115.1 / 115.1 / 119.2).
+constexpr int KV_JOIN = 8;
+template <int QT>
+constexpr int KV_GROUP = QT == 2 ? 8 : 16;
 
 // parts first, first + step, ... (count of them; number i stands in slot_of(i), its maxima and sums `stats` floats into it) ->
 // the result, or one part, in the slot of `first`, its maxima and sums in the second place for them
-template <typename T, int HD, int NW, typename SlotOf>
+template <typename T, int HD, int NW, int QT, typename SlotOf>
 __device__ __forceinline__ void kv_reduce(const KvAttend &a, float *lds, int s, int hq0, int rows, SlotOf slot_of, int first, int step, int count,
                                           int stats, bool result) {
-    constexpr int NTH = NW * 64;
-    const __amdgpu_buffer_rsrc_t parts = kv_partials(a);
+    constexpr int NTH = NW * 64, R = 16 * QT, SLOT = kv_slot(HD, QT);
+    const __amdgpu_buffer_rsrc_t parts = kv_partials<HD, QT>(a);
     const int quads = rows * (HD / 4);
     const int lanes = min(max(NTH / quads, 1), count);   // threads that share four columns
     for (int e0 = 0; e0 < quads; e0 += NTH / lanes) {
@@ -548,24 +591,23 @@ __device__ __forceinline__ void kv_reduce(const KvAttend &a, float *lds, int s, 
 #pragma unroll
             for (int i = 0; i < KV_JOIN; ++i) {
                 const bool there = i0 + i * lanes < count;
-                const int p = slot_of(first + (there ? i0 + i * lanes : i0) * step) * kv_slot(HD);
-                m[i] = kv_get(parts, p + stats + r), l[i] = kv_get(parts, p + stats + 16 + r);
-                o[i] = kv_get4(parts, p + 64 + r * HD + d);
+                const int p = slot_of(first + (there ? i0 + i * lanes : i0) * step) * SLOT;
+                m[i] = kv_get(parts, p + stats + r), l[i] = kv_get(parts, p + stats + R + r);
+                o[i] = kv_get4(parts, p + 4 * R + r * HD + d);
             }
+            __builtin_amdgcn_sched_barrier(0);   // (else the first maxima are waited for before the last loads are on their way)
             float mn = mm;
 #pragma unroll
-            for (int i = 0; i < KV_JOIN; ++i) mn = fmaxf(mn, m[i]);   // (one that stands in for a missing part changes nothing)
+            for (int i = 0; i < KV_JOIN; ++i) mn = fmaxf(mn, m[i]);   // (one that stands in for a missing part changes nothing, then weighs nothing)
             const float c = __builtin_amdgcn_exp2f((mm - mn) * KV_LOG2E);
             sum *= c, acc *= c, mm = mn;
 #pragma unroll
             for (int i = 0; i < KV_JOIN; ++i) {
                 const bool there = i0 + i * lanes < count;
-                const float w = __builtin_amdgcn_exp2f((m[i] - mm) * KV_LOG2E);
-                if (there) {
-                    sum = fmaf(l[i], w, sum);
+                const float w = there ? __builtin_amdgcn_exp2f((m[i] - mm) * KV_LOG2E) : 0.f;
+                sum = fmaf(l[i], w, sum);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) acc[x] = fmaf(o[i][x], w, acc[x]);
-                }
+                for (int x = 0; x < 4; ++x) acc[x] = fmaf(o[i][x], w, acc[x]);
             }
         }
         if (lanes > 1) {
@@ -593,9 +635,9 @@ __device__ __forceinline__ void kv_reduce(const KvAttend &a, float *lds, int s, 
                 kv_result<T>(a, s, hq0 + r, d, acc);
                 if (a.lse && d == 0) a.lse[(int64_t)s * a.n_q_heads + hq0 + r] = mm + logf(sum);
             } else {   // (only this thread reads these columns of the slot; its maxima others may still read)
-                const int p = slot_of(first) * kv_slot(HD);
-                kv_put(parts, p + 64 + r * HD + d, acc);
-                if (d == 0) kv_put(parts, p + 32 + r, mm), kv_put(parts, p + 48 + r, sum);
+                const int p = slot_of(first) * SLOT;
+                kv_put(parts, p + 4 * R + r * HD + d, acc);
+                if (d == 0) kv_put(parts, p + 2 * R - stats + r, mm), kv_put(parts, p + 3 * R - stats + r, sum);
             }
         }
     }
@@ -617,46 +659,50 @@ __device__ __forceinline__ bool kv_last(int32_t *counter, int of, float *lds) {
     return is;
 }
 
-template <typename T, int HD, int NW>
+template <typename T, int HD, int NW, int QT>
 __device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, int pair, int first_wg, int n_parts) {
     const int h = pair / a.q_tiles, qt = pair % a.q_tiles;
-    const int hq0 = h * a.group + qt * 16, rows = min(16, a.group - qt * 16);
+    constexpr int R = 16 * QT;
+    const int hq0 = h * a.group + qt * R, rows = min(R, a.group - qt * R);
     // the first part stands in the slot of a segment that goes on, the others in that of one that came from before
     const auto slot_of = [&](int i) { return 2 * (first_wg + i) + (i == 0 ? 1 : 0); };
-    const bool grouped = n_parts > 2 * KV_GROUP;
-    int first = grouped ? (int)(blockIdx.x - first_wg) / KV_GROUP * KV_GROUP : 0;
-    int count = grouped ? min(KV_GROUP, n_parts - first) : n_parts, step = 1;
-    int32_t *counter = a.counters + slot_of(first);
-    while (kv_last(counter, count, lds)) {
-        const bool result = !grouped || step > 1;
-        kv_reduce<T, HD, NW>(a, lds, s, hq0, rows, slot_of, first, step, count, step > 1 ? 32 : 0, result);
+    constexpr int G = KV_GROUP<QT>;
+    static_assert(2 * G * G * G >= WT_KV_WORKSPACE_ZEROED / 16, "parts of one pair: a workgroup each");
+    const int i = blockIdx.x - first_wg;
+    for (int level = 0, step = 1;; ++level, step *= G) {
+        const int left = (n_parts + step - 1) / step;   // parts 0, step, 2 * step ... are still to be joined
+        const bool result = left <= 2 * G;
+        const int first = result ? 0 : i / (step * G) * G, count = result ? left : min(G, left - first);
+        // counters of this pair's own: level 0 in the first half, the others in the second (those of level 1 at multiples of G * G);
+        // level 2 is the last
+        int32_t *counter = a.counters + (level == 0 ? 0 : 2 * a.n_wg) + slot_of(level < 2 ? first * step : 1);
+        if (!kv_last(counter, count, lds)) return;
+        kv_reduce<T, HD, NW, QT>(a, lds, s, hq0, rows, slot_of, first * step, step, count, level & 1 ? 2 * R : 0, result);
         if (result) return;
-        first = 0, step = KV_GROUP, count = (n_parts + KV_GROUP - 1) / KV_GROUP;
-        counter = a.counters + 2 * a.n_wg + slot_of(0);
     }
 }
 
 // Short tables: one workgroup per (sequence, key head, query tile).  One head is bound by what a compute unit streams and by the
 // chain length -> table -> keys -> joining waves (447 keys of 8 heads, f16, 64 values: 6.3 us), many by memory (32 sequences of 1500, 20
 // heads: 45 us, 5.4 TB/s).
-template <typename CT, typename T, int HD, int PG, int NW>
-__global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_direct_kernel(const KvAttend a) {
+template <typename CT, typename T, int HD, int PG, int NW, int QT>
+__global__ __launch_bounds__(NW * 64, HD * QT <= 128 ? 2 : 1) void kv_attend_direct_kernel(const KvAttend a) {
     extern __shared__ __attribute__((aligned(16))) float kv_lds[];
     const unsigned pairs = a.c.n_heads * a.q_tiles;
-    KvWave<CT, T, HD, PG, NW> w(a);
-    kv_segment<true, CT, T, HD, PG, NW>(w, a, kv_lds, blockIdx.x / pairs, blockIdx.x % pairs, 0, false, 0, 0, -1);
+    KvWave<CT, T, HD, PG, NW, QT> w(a);
+    kv_segment<true, CT, T, HD, PG, NW, QT>(w, a, kv_lds, blockIdx.x / pairs, blockIdx.x % pairs, 0, false, 0, 0, -1);
 }
 
 // Longer ones: one workgroup a compute unit, equal shares.  Bound by memory; 131071 positions of 8 heads, bf16, 128 values: 90.5 us (5.9
 // TB/s), 16 sequences of 17 ... 32768: 62.5 us (5.5), 4 of 50001 ... 65537 in 8 bits: 82 us (5.8).  Two workgroups a compute unit
 // progress unevenly: their ends lay between 55 and 106 us where one's lay between 76 and 99.
-template <typename CT, typename T, int HD, int PG, int NW>
-__global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_kernel(const KvAttend a) {
+template <typename CT, typename T, int HD, int PG, int NW, int QT>
+__global__ __launch_bounds__(NW * 64, HD * QT <= 128 ? 2 : 1) void kv_attend_kernel(const KvAttend a) {
     extern __shared__ __attribute__((aligned(16))) float kv_lds[];
     constexpr int KB = KvKind<CT, T, HD>::KB, UNIT = KB * NW;
     const int lane = threadIdx.x & 63;
     const int pairs = a.c.n_heads * a.q_tiles;   // of one sequence
-    KvWave<CT, T, HD, PG, NW> w(a);
+    KvWave<CT, T, HD, PG, NW, QT> w(a);
     // All pairs stand in a row, sequence by sequence, each with seg_cost units for what a segment costs by itself (queries,
     // joining the waves) and then one for every NW blocks of keys; workgroup i takes the i-th share of the row.
     const int n_seqs = a.t.n_seqs, head = a.seg_cost;
@@ -714,10 +760,10 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_kernel(c
         if (n == 0 ? u == p0 : to > from) {   // (an empty sequence belongs to the workgroup that holds its first unit)
             const bool whole = from == 0 && to == n;
             const int slot = whole ? -1 : 2 * (int)blockIdx.x + (from == 0 ? 1 : 0);
-            kv_segment<false, CT, T, HD, PG, NW>(w, a, kv_lds, s, pair, len, wrong, from * NW, min(to * NW, (len + KB - 1) / KB), slot);
+            kv_segment<false, CT, T, HD, PG, NW, QT>(w, a, kv_lds, s, pair, len, wrong, from * NW, min(to * NW, (len + KB - 1) / KB), slot);
             if (!whole) {
                 const int first_wg = (int)kv_div(k0, share), last_wg = (int)kv_div(k0 + n - 1, share);
-                kv_join<T, HD, NW>(a, kv_lds, s, pair, first_wg, last_wg - first_wg + 1);
+                kv_join<T, HD, NW, QT>(a, kv_lds, s, pair, first_wg, last_wg - first_wg + 1);
             }
             __syncthreads();   // lds is free
         }
@@ -728,13 +774,15 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void kv_attend_kernel(c
 
 template <typename CT, typename T, int HD, int PG>
 static int kv_attend_go(const KvAttend &a, unsigned grid, hipStream_t st) {
-    const int rows = a.group < 16 ? a.group : 16;
-    void (*kernel)(KvAttend) = !a.direct     ? kv_attend_kernel<CT, T, HD, PG, KV_WAVES>
-                               : a.waves == 2 ? kv_attend_direct_kernel<CT, T, HD, PG, 2>
-                                              : kv_attend_direct_kernel<CT, T, HD, PG, KV_WAVES>;
-    size_t lds = sizeof(float) * a.waves * (32 + (size_t)rows * HD);
+    const int tile = 16 * a.q_wide, rows = a.group < tile ? a.group : tile;
+    void (*kernel)(KvAttend) = !a.direct     ? kv_attend_kernel<CT, T, HD, PG, KV_WAVES, 1>
+                               : a.waves == 2 ? kv_attend_direct_kernel<CT, T, HD, PG, 2, 1>
+                                              : kv_attend_direct_kernel<CT, T, HD, PG, KV_WAVES, 1>;
+    if constexpr (HD <= KV_WIDE_HD)
+        if (a.q_wide == 2) kernel = a.direct ? kv_attend_direct_kernel<CT, T, HD, PG, KV_WAVES, 2> : kv_attend_kernel<CT, T, HD, PG, KV_WAVES, 2>;
+    size_t lds = sizeof(float) * a.waves * (2 * tile + (size_t)rows * HD);
     if (!a.direct && lds < sizeof(float) * KV_WAVES * 64 * 6) lds = sizeof(float) * KV_WAVES * 64 * 6;   // what the join of partial results takes
-    if (lds > 64 * 1024)   // (16 queries of 256 values)
+    if (lds > 64 * 1024)   // (16 queries of 256 values, 32 of 128)
         WT_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * a.waves), lds, st, a);
     WT_HIP(hipGetLastError());
