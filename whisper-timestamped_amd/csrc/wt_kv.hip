@@ -341,25 +341,29 @@ static int kv_plan(const wt_kv_cache *c, int n_seqs, int n_q_heads, int table_wi
     const int64_t heads = (int64_t)n_seqs * c->n_heads, narrow = heads * ((group + 15) / 16);
     const int64_t key_bytes = 2ll * c->head_dim * (c->dtype == WT_DTYPE_F32 ? 4 : c->dtype == WT_DTYPE_E4M3 ? 1 : 2);   // and its value's
     p->n_wg = n < WT_KV_WORKSPACE_ZEROED / 16 ? n : WT_KV_WORKSPACE_ZEROED / 16;   // (four counters each)
-    // A share is at least two units (blocks of KV_WAVES waves: 16 to 64 KB), one of 128 KB: 8 pairs of 512 KB, 1 / 2 / 4 units: f16, 64
-    // values 13.6 / 11.9 / 13.3 us, bf16, 128 values 13.7 / 13.7 / 17.1, 256 values 16.7 / 20.5 / 25.4.  A segment of its own costs about two
-    // (16 sequences up to 32768, without / 2 / 4 / 8: 107 / 64 / 65 / 68 us).
-    p->min_share = key_bytes * KV_WAVES * (c->dtype == WT_DTYPE_F32 ? 16 : 32) >= 128 * 1024 ? 1 : 2;
+    const int64_t unit = key_bytes * KV_WAVES * (c->dtype == WT_DTYPE_F32 ? 16 : 32);   // a block of each of KV_WAVES waves: 8 to 128 KB
+    p->min_share = unit < 32 * 1024 ? 2 : 1;
+    // A segment of its own costs about two units (16 sequences up to 32768, without / 2 / 4 / 8: 107 / 64 / 65 / 68 us).
     p->seg_cost = 2;
     // One workgroup streams keys and values at some 48 GB/s whatever its waves (four 8.8 us, eight 9.7, sixteen 11.5 over 250 KB), and
-    // splitting them costs about 6 us.  Direct / shares, us: 8 and 32 pairs (f16, 64 values) of 256 KB 8.8 / 10.3 and 9.7 / 11.1, of 384 KB
-    // 11.5 / 11.4 and 13.5 / 12.1, of 512 KB 14.2 / 11.8 and 16.7 / 13.1; 128 pairs of 512 KB 19.0 / 18.7; 256 of 512 KB 22.8 / 24.6.
+    // splitting them costs 3 to 5 us.  Direct / shares, us: 8 and 32 heads of 192, 256 and 384 KB: f16, 64 values (units of 32 KB) 7.4 / 7.7,
+    // 8.8 / 8.1, 11.5 / 8.9 and 7.7 / 8.6, 9.6 / 9.5, 13.4 / 9.7; bf16, 128 values (64 KB) 8.0 / 9.9, 9.3 / 10.4, 11.4 / 10.5 and 8.7 / 11.1, 10.7 /
+    // 11.3, 14.3 / 11.5; 128 heads of 256, 384 and 512 KB: 11.2 / 13.0, 15.1 / 15.3, 18.9 / 18.0 and 12.5 / 16.3, 16.5 / 18.5, 20.3 / 20.8; 256
+    // heads of 512 KB 22.8 / 24.3 and 24.7 / 26.5.
     const int64_t capacity = (int64_t)table_width * c->page_size * key_bytes;
-    const auto is_direct = [&](int64_t pairs) { return capacity <= (pairs <= n / 4 ? 384 : 512) * 1024 && pairs <= KV_MAX_GRID; };
+    const auto is_direct = [&](int64_t pairs) {
+        const int64_t kb = unit <= 32 * 1024 ? (pairs <= n / 4 ? 208 : pairs <= n / 2 ? 384 : 512) : pairs <= n / 4 ? 320 : 512;
+        return capacity <= kb * 1024 && pairs <= KV_MAX_GRID;
+    };
     // More than 16 query heads a key head: 32 at a time read keys and values half as often, but leave one wave a SIMD where a key is more than
     // 64 values of 16 bits, and their partial results are twice as long.  16 / 32 at a time, us, 24 query heads a key head.  Whole tables of
     // 448 keys, 128, 256 and 384 tiles of 16: bf16, 128 values 12.5 / 14.1, 14.5 / 14.8, 23.2 / 15.5, f32, 64 values 11.7 / 13.7, 13.1 /
     // 14.0, 21.0 / 14.4.  5120 tiles of 32, 128, 224, 448 keys: bf16, 128 values 41 / 59, 86 / 85, 117 / 102, 188 / 137, 96 values 30 / 53, 49 /
     // 65, 73 / 81, 125 / 106, 8 bits, 128 values 34 / 60, 50 / 71, 65 / 82, 104 / 102; f16, 64 values 21 / 21, 44 / 31, 59 / 40, 94 / 58, f32, 64
-    // values 39 / 27 ... 179 / 106, 128 values 81 / 76 ... 402 / 238.  Shares, tables of 50, 100, 300 (8 bits) or 600 MB in all: bf16, 128 values
-    // 28.7 / 33.3, 47 / 41, 195 / 115, f16, 64 values 25.2 / 25.4, 40 / 35, 100 / 62, 8 bits, 128 values 33 / 35, 48 / 49, 107 / 77.
+    // values 39 / 27 ... 179 / 106, 128 values 81 / 76 ... 402 / 238.  Shares, tables of 50, 100 and 300 (8 bits) or 600 MB in all: bf16, 128 values
+    // 24.0 / 26.3, 41.5 / 33.6, 193 / 109, f16, 64 values 22.8 / 21.5, 37.7 / 30.8, 99 / 58, 8 bits, 128 values 28.0 / 28.5, 42.6 / 40.5, 106 / 73.
     const bool widen = is_direct(narrow) ? narrow > n && (c->head_dim <= 64 || c->dtype == WT_DTYPE_F32 || capacity >= 128 * 1024)
-                                         : heads * capacity >= 80 * 1024 * 1024;
+                                         : heads * capacity >= 64 * 1024 * 1024;
     p->q_wide = group > 16 && c->head_dim <= KV_WIDE_HD && widen ? 2 : 1;
     p->q_tiles = (group + 16 * p->q_wide - 1) / (16 * p->q_wide);
     const int64_t pairs = heads * p->q_tiles;

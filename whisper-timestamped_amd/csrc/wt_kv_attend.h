@@ -562,10 +562,10 @@ __device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW, QT> &w, con
 }
 
 // The last workgroup of a pair to arrive joins its partial results.  A thread takes four columns of a row, and where there
-// are more threads than that, every LANES-th part; KV_JOIN parts are loaded at a time, in an order that never changes.  One workgroup
-// reads partial results at some 48 GB/s, so with more than two KV_GROUPs of parts the last of each group joins the group, and the
-// last of those the groups, and so on (90 parts of 8 queries of 256 values: 30 us by one workgroup alone; 24 queries of 128 values,
-// 8 heads of 12000 positions, groups of 16 / 12 / 8 / 6: 43.6 / 38.1 / 33.3 / 33.2 us, of 40000 114.9 / 115.1 / 115.1 / 119.2).
+// are more threads than that and more than KV_JOIN parts, every LANES-th part; KV_JOIN parts are loaded at a time, in an order
+// that never changes.  One workgroup reads partial results at some 48 GB/s, so with more than two KV_GROUPs of parts the last of
+// each group joins the group, and the last of those the groups, and so on (90 parts of 8 queries of 256 values: 30 us by one
+// workgroup alone; 24 queries of 128 values over 24000 and 48000 positions of 8 heads, groups of 16 / 8: 36.3 / 33.6, 54.2 / 51.4 us).
 constexpr int KV_JOIN = 8;
 template <int QT>
 constexpr int KV_GROUP = QT == 2 ? 8 : 16;
@@ -578,7 +578,7 @@ __device__ __forceinline__ void kv_reduce(const KvAttend &a, float *lds, int s, 
     constexpr int NTH = NW * 64, R = 16 * QT, SLOT = kv_slot(HD, QT);
     const __amdgpu_buffer_rsrc_t parts = kv_partials<HD, QT>(a);
     const int quads = rows * (HD / 4);
-    const int lanes = min(max(NTH / quads, 1), count);   // threads that share four columns
+    const int lanes = min(max(NTH / quads, 1), (count + KV_JOIN - 1) / KV_JOIN);   // threads that share four columns
     for (int e0 = 0; e0 < quads; e0 += NTH / lanes) {
         const int e = e0 + threadIdx.x / lanes, mine = threadIdx.x % lanes;
         const bool in = e < quads && threadIdx.x / lanes < NTH / lanes;
@@ -595,7 +595,8 @@ __device__ __forceinline__ void kv_reduce(const KvAttend &a, float *lds, int s, 
                 m[i] = kv_get(parts, p + stats + r), l[i] = kv_get(parts, p + stats + R + r);
                 o[i] = kv_get4(parts, p + 4 * R + r * HD + d);
             }
-            __builtin_amdgcn_sched_barrier(0);   // (else the first maxima are waited for before the last loads are on their way)
+            __builtin_amdgcn_sched_barrier(0);   // (else maxima are waited for before the last loads are on their way: 37.7 instead of 27.1 us
+                                                 // for 131072 positions of one head with 16 queries)
             float mn = mm;
 #pragma unroll
             for (int i = 0; i < KV_JOIN; ++i) mn = fmaxf(mn, m[i]);   // (one that stands in for a missing part changes nothing, then weighs nothing)
@@ -693,8 +694,8 @@ __global__ __launch_bounds__(NW * 64, HD * QT <= 128 ? 2 : 1) void kv_attend_dir
     kv_segment<true, CT, T, HD, PG, NW, QT>(w, a, kv_lds, blockIdx.x / pairs, blockIdx.x % pairs, 0, false, 0, 0, -1);
 }
 
-// Longer ones: one workgroup a compute unit, equal shares.  Bound by memory; 131071 positions of 8 heads, bf16, 128 values: 90.5 us (5.9
-// TB/s), 16 sequences of 17 ... 32768: 62.5 us (5.5), 4 of 50001 ... 65537 in 8 bits: 82 us (5.8).  Two workgroups a compute unit
+// Longer ones: one workgroup a compute unit, equal shares.  Bound by memory; 131071 positions of 8 heads, bf16, 128 values: 88 us (6.1
+// TB/s), 16 sequences of 17 ... 32768: 61 us (5.6), 4 of 50001 ... 65537 in 8 bits: 80 us (5.9).  Two workgroups a compute unit
 // progress unevenly: their ends lay between 55 and 106 us where one's lay between 76 and 99.
 template <typename CT, typename T, int HD, int PG, int NW, int QT>
 __global__ __launch_bounds__(NW * 64, HD * QT <= 128 ? 2 : 1) void kv_attend_kernel(const KvAttend a) {
