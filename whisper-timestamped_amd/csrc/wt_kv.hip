@@ -7,7 +7,7 @@ namespace wt {
 
 // ---- writing rows and reading them back -----------------------------------------------------------------------------
 // A row (one head of one token) is HD values; LPR lanes take EPL = HD / LPR of them each, so that a lane moves 16 bytes
-// outside of the cache (24 or 12 where a row is 96 values).  A workgroup takes KV_RT consecutive rows of the call, slots
+// outside of the cache (24 or 12 where a row is 96 values).  A workgroup takes up to 16 consecutive rows of the call, slots
 // innermost: rows of a prompt that share a line of the cache (64 values of 8 bits: two a line) are written by one
 // workgroup, and every lane group moves whole runs of 64 ... 256 bytes on both sides.  Both directions are bound by memory:
 // a lane finds its row's place once and has KV_HU heads' keys and values in flight, past the caches (one head, plain loads: 35 / 168 /
