@@ -4,6 +4,7 @@
 #include <hip/hip_fp16.h>
 
 #include "wt_common.h"
+#include "wt_kv_plan.h"
 
 namespace wt {
 

@@ -566,7 +566,6 @@ __device__ __forceinline__ void kv_segment(KvWave<CT, T, HD, PG, NW, QT> &w, con
 // that never changes.  One workgroup reads partial results at some 48 GB/s, so with more than two KV_GROUPs of parts the last of
 // each group joins the group, and the last of those the groups, and so on (90 parts of 8 queries of 256 values: 30 us by one
 // workgroup alone; 24 queries of 128 values over 24000 and 48000 positions of 8 heads, groups of 16 / 8: 36.3 / 33.6, 54.2 / 51.4 us).
-constexpr int KV_JOIN = 8;
 template <int QT>
 constexpr int KV_GROUP = QT == 2 ? 8 : 16;
 
@@ -578,10 +577,10 @@ __device__ __forceinline__ void kv_reduce(const KvAttend &a, float *lds, int s, 
     constexpr int NTH = NW * 64, R = 16 * QT, SLOT = kv_slot(HD, QT);
     const __amdgpu_buffer_rsrc_t parts = kv_partials<HD, QT>(a);
     const int quads = rows * (HD / 4);
-    const int lanes = min(max(NTH / quads, 1), (count + KV_JOIN - 1) / KV_JOIN);   // threads that share four columns
+    const int lanes = kv_join_lanes(NTH, quads, count);
     for (int e0 = 0; e0 < quads; e0 += NTH / lanes) {
         const int e = e0 + threadIdx.x / lanes, mine = threadIdx.x % lanes;
-        const bool in = e < quads && threadIdx.x / lanes < NTH / lanes;
+        const bool in = e < quads && kv_join_grouped(threadIdx.x, lanes, NTH);
         const int r = in ? e / (HD / 4) : 0, d = in ? e % (HD / 4) * 4 : 0;
         float mm = KV_LOWEST, sum = 0.f;
         f4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -617,7 +616,7 @@ __device__ __forceinline__ void kv_reduce(const KvAttend &a, float *lds, int s, 
 #pragma unroll
             for (int x = 0; x < 4; ++x) mine_lds[2 + x] = acc[x];
             __syncthreads();
-            if (mine == 0)
+            if (in && mine == 0)
                 for (int i = 1; i < lanes; ++i) {
                     const float *p = mine_lds + 6 * i;
                     const float mn = fmaxf(mm, p[0]);
