@@ -79,10 +79,10 @@ class PagedText:
             wv = attn.qkv_attention(q, k, v, mask)[0]
         else:
             raise WtError(f"paged text: {n_new} tokens at once behind {self.past}: only a loop's first call holds several")
-        if layer == len(self.caches) - 1:
-            self.past += n_new
         if layer == 0:       # what the backend's decoder takes its offset from: the first entry's second dimension
             kv_cache[attn.key] = x.new_empty(1).expand(batch, self.past + n_new, state)
+        if layer == len(self.caches) - 1:       # (behind the line above: the first layer may be the last)
+            self.past += n_new
         return attn.out(wv), None
 
     def _install_kv_cache_hooks(self, original, cache=None):
