@@ -67,3 +67,20 @@ def test_decoders_of_any_depth(layers, prompt_len, monkeypatch):
         # two orders of the same 32-bit sums: a few hundred roundings of 2^-24 a layer, logits of about 10; a wrong position
         # is off by 10 and more
         assert float((got - want).abs().max()) <= 2.0 ** -24 * 512 * layers * float(want.abs().max())
+
+
+def test_a_model_is_attached_once(monkeypatch):
+    """A second block over the same model is refused, and the first one still leaves the model as it was."""
+    from whisper_timestamped import paged_decoder
+    from whisper_timestamped._lib import WtError
+    monkeypatch.setattr(paged_decoder, "PagedKVCache", PlainCache)
+    model = small_model(2)
+    one, two = (paged_decoder.PagedText(model, 1, torch.float32) for _ in range(2))
+    with one.attached():
+        with pytest.raises(WtError, match="attached"), two.attached():
+            pass
+        assert not paged_decoder.supported(model, torch.float32)
+    assert "install_kv_cache_hooks" not in vars(model) and not any("forward" in vars(b.attn) for b in model.decoder.blocks)
+    with two.attached():
+        pass
+    assert paged_decoder.supported(model, torch.float32)

@@ -20,11 +20,14 @@ from .kvcache import HEAD_DIMS, PagedKVCache
 PAGE = 32
 
 
+def _replaced(model) -> bool:
+    return any("forward" in vars(b.attn) for b in model.decoder.blocks) or "install_kv_cache_hooks" in vars(model)
+
+
 def supported(model, dtype) -> bool:
     dims = model.dims
     return dims.n_text_state // dims.n_text_head in HEAD_DIMS and dtype in (torch.float16, torch.float32, torch.bfloat16) and \
-        not any("forward" in vars(b.attn) for b in model.decoder.blocks) and "install_kv_cache_hooks" not in vars(model) and \
-        all(hasattr(b.attn, m) for b in model.decoder.blocks for m in ("query", "key", "value", "out", "qkv_attention"))
+        not _replaced(model) and all(hasattr(b.attn, m) for b in model.decoder.blocks for m in ("query", "key", "value", "out", "qkv_attention"))
 
 
 class PagedText:
@@ -102,6 +105,8 @@ class PagedText:
     def attached(self):
         """For one decoder loop."""
         m = self.model
+        if _replaced(m):
+            raise WtError("paged text: the model's attention or cache hooks are replaced already (attached twice?)")
         blocks = list(m.decoder.blocks)
         install = m.install_kv_cache_hooks
         m.install_kv_cache_hooks = lambda cache=None: self._install_kv_cache_hooks(install, cache)
