@@ -25,6 +25,7 @@ struct KvKind {
     static constexpr int NT = KB / 16;                      // ... in tiles of 16
     static constexpr int GK = KB / 4;                       // keys a lane group holds the weights and values of
     static constexpr int QP = !E4M3 ? 1 : __is_same(T, bf16_t) ? 1 : __is_same(T, f16_t) ? 2 : 3;
+    static constexpr int WP = sizeof(T) == 4 ? 3 : 2;       // 16-bit parts of a weight: as many bits as the results hold, and 9 at least to spare
     // f16 weights are kept away from f16's subnormal numbers: the reference of the exponentials sits BIAS below the maximum
     // seen, which may be outgrown by SLACK before it moves; exp(BIAS + SLACK) < 65504
     static constexpr float BIAS = F16 ? 5.5f : 0.f, SLACK = F16 ? 5.5f : 8.f;
@@ -227,6 +228,11 @@ struct KvWave {
         if constexpr (K::F16) return (float)__builtin_bit_cast(h2, w).y;
         else return __uint_as_float(w & 0xffff0000u);
     }
+    static __device__ __forceinline__ uint32_t part(float &x, float &y) {   // the next 16-bit part of two numbers, which become what is left of them
+        const uint32_t w = pack16(x, y);
+        x -= low16(w), y -= high16(w);
+        return w;
+    }
 
     // One block of KB keys.  Scores as (keys x queries) tiles: A rows are keys, chosen so that lane group g gets keys g * GK
     // ... + GK - 1 of its query (column n) in order; they are, without leaving the lane, the B operand of (values^T x
@@ -329,17 +335,18 @@ struct KvWave {
 #pragma unroll
                     for (int y = 0; y < QT; ++y) o[y][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[j][i]), p[y][j], o[y][i], 0, 0, 0);
         } else {
-            // a weight is the sum of two 16-bit numbers: with one alone the result is off by up to 2^-8 (bf16) where few keys
-            // share the weight; with both by less than 2^-16
-            // values arrive as rows (key j: EV neighbouring columns a lane) and are needed as columns: pairs of rows are
-            // interleaved by byte permutes
-            u4 hi[QT], lo[QT];
+            // A weight is the sum of WP 16-bit numbers: with one alone a result is off by up to 2^-8 (bf16) where few keys share the weight, with
+            // two by less than 2^-16, which 16-bit results do not show; f32 results (over 8-bit pages) take three, all 24 bits.
+            // Values arrive as rows (key j: EV neighbouring columns a lane) and are needed as columns: pairs of rows are
+            // interleaved by byte permutes.
+            u4 weight[QT][K::WP];
 #pragma unroll
             for (int y = 0; y < QT; ++y)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    hi[y][i] = pack16(p[y][2 * i], p[y][2 * i + 1]);
-                    lo[y][i] = pack16(p[y][2 * i] - low16(hi[y][i]), p[y][2 * i + 1] - high16(hi[y][i]));
+                    float w0 = p[y][2 * i], w1 = p[y][2 * i + 1];
+#pragma unroll
+                    for (int n = 0; n < K::WP; ++n) weight[y][n][i] = part(w0, w1);
                 }
             uint32_t w[8][EV / 2];
 #pragma unroll
@@ -351,14 +358,15 @@ struct KvWave {
                 }
 #pragma unroll
             for (int i = 0; i < EV; ++i) {
+                if constexpr (K::WP > 2) __builtin_amdgcn_sched_barrier(0);   // (columns in turn: registers for one more wave a SIMD; 128 short tables 12.8 -> 12.3 us)
                 u4 vt;
 #pragma unroll
                 for (int jj = 0; jj < 4; ++jj)
                     vt[jj] = __builtin_amdgcn_perm(w[2 * jj + 1][i / 2], w[2 * jj][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                for (int y = 0; y < QT; ++y) o[y][i] = mma(vt, lo[y], o[y][i]);
+                for (int n = K::WP - 1; n >= 0; --n)
 #pragma unroll
-                for (int y = 0; y < QT; ++y) o[y][i] = mma(vt, hi[y], o[y][i]);
+                    for (int y = 0; y < QT; ++y) o[y][i] = mma(vt, weight[y][n], o[y][i]);
             }
         }
     }
@@ -403,11 +411,7 @@ struct KvWave {
 #pragma unroll
                     for (int p = 0; p < K::QP; ++p)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t w = pack16(v[2 * i], v[2 * i + 1]);
-                            q[y][p][st][i] = w;
-                            v[2 * i] -= low16(w), v[2 * i + 1] -= high16(w);
-                        }
+                        for (int i = 0; i < 4; ++i) q[y][p][st][i] = part(v[2 * i], v[2 * i + 1]);
                 }
             }
         }
