@@ -348,7 +348,7 @@ WT_API int wt_kv_gather(const wt_kv_cache *cache, void *k, void *v, int dtype, i
  *     w_t = scale * q . k_t,   out = sum_t exp(w_t - max w) v_t / sum_t exp(w_t - max w),   lse = log sum_t exp(w_t)
  * Products are summed, and maximum, sum and result held, in 32 bits; a weight takes part with 24 bits where out is f32, with 16 where it has
  * 16 bits itself; out is rounded once.  lengths[s] = 0: out = 0, lse = -inf.  What pages hold behind the last position takes no part, NaN and infinities included; an infinity among the values
- * that do take part leaves its element infinite or NaN.  Sums of values run up to exp(11) * sum |v_t| before they are divided: where
+ * that do take part leaves its element infinite or NaN.  Sums of values run up to exp(8) * sum |v_t| before they are divided: where
  * that is beyond 2^128 the result is not finite, and of values below 2^-100 bits are lost.
  *   q, out : device, dtype F32 / F16 / BF16 (the cache's own; any of them over an E4M3 cache), head_dim values in a row;
  *            out may be q.  Rows beyond n_seqs are not touched

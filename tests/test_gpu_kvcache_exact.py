@@ -30,10 +30,8 @@ def cache_of(k, v, page, dtype, exponents=(127, 127)):
     return PagedKVCache(*both, *e), order.int().to(DEV)[None]
 
 
-WEIGHTS = [(q, d, n, s) for q, d in PAIRS for n, s in ((1, 0.0), (2, 1.0), (31, 3.5), (64, 3.5), (64, 20.0)) if d != F16 or s < 20.0]
-
-
-@pytest.mark.parametrize("q_dtype,dtype,n,spread", WEIGHTS)
+@pytest.mark.parametrize("n,spread", [(1, 0.0), (2, 1.0), (31, 3.5), (64, 3.5), (64, 20.0)])
+@pytest.mark.parametrize("q_dtype,dtype", PAIRS)
 def test_each_weight_by_itself(q_dtype, dtype, n, spread):
     """Key t has a value in column t alone, so element t of the result is its weight: each has as many bits as the result's type,
     also one that is e^-20 of the largest.  Scores are single products, exact."""

@@ -25,10 +25,10 @@ struct KvKind {
     static constexpr int NT = KB / 16;                      // ... in tiles of 16
     static constexpr int GK = KB / 4;                       // keys a lane group holds the weights and values of
     static constexpr int QP = !E4M3 ? 1 : __is_same(T, bf16_t) ? 1 : __is_same(T, f16_t) ? 2 : 3;
-    static constexpr int WP = sizeof(T) == 4 ? 3 : 2;       // 16-bit parts of a weight: as many bits as the results hold, and 9 at least to spare
-    // f16 weights are kept away from f16's subnormal numbers: the reference of the exponentials sits BIAS below the maximum
-    // seen, which may be outgrown by SLACK before it moves; exp(BIAS + SLACK) < 65504
-    static constexpr float BIAS = F16 ? 5.5f : 0.f, SLACK = F16 ? 5.5f : 8.f;
+    // The second product is one of bf16 operands for every page type but f32: a weight is the sum of WP bf16 numbers (as many bits as results
+    // hold, and 5 more at least), an f16 value of two, exactly; a bf16 value and an 8-bit code are one
+    static constexpr int WP = sizeof(T) == 4 ? 3 : 2, VP = F16 ? 2 : 1;
+    static constexpr float SLACK = 8.f;   // by what the running maximum may be outgrown before it moves
 };
 
 // d index of the first of the 8 (f32: 4) elements that lane group g takes of contraction step s; K and Q use the same one.
@@ -207,30 +207,22 @@ struct KvWave {
         }
     }
 
-    static __device__ __forceinline__ f4 mma(u4 x, u4 y, f4 c) {
+    static __device__ __forceinline__ f4 mma_bf16(u4 x, u4 y, f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, x), __builtin_bit_cast(bf8, y), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f4 mma(u4 x, u4 y, f4 c) {   // of operands as pages and queries hold them
         if constexpr (K::F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
-        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, x), __builtin_bit_cast(bf8, y), c, 0, 0, 0);
+        else return mma_bf16(x, y, c);
     }
     static __device__ __forceinline__ uint32_t codes(uint32_t w, bool high) {   // two 8-bit codes as bf16
         return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, true))
                     : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, false));
     }
-    static __device__ __forceinline__ uint32_t pack16(float x, float y) {
+    // the next bf16 part of two numbers, which become what is left of them
+    static __device__ __forceinline__ uint32_t part(float &x, float &y) {
         const fl2 v = {x, y};
-        if constexpr (K::F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
-        else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf2));
-    }
-    static __device__ __forceinline__ float low16(uint32_t w) {
-        if constexpr (K::F16) return (float)__builtin_bit_cast(h2, w).x;
-        else return __uint_as_float(w << 16);
-    }
-    static __device__ __forceinline__ float high16(uint32_t w) {
-        if constexpr (K::F16) return (float)__builtin_bit_cast(h2, w).y;
-        else return __uint_as_float(w & 0xffff0000u);
-    }
-    static __device__ __forceinline__ uint32_t part(float &x, float &y) {   // the next 16-bit part of two numbers, which become what is left of them
-        const uint32_t w = pack16(x, y);
-        x -= low16(w), y -= high16(w);
+        const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf2));
+        x -= __uint_as_float(w << 16), y -= __uint_as_float(w & 0xffff0000u);
         return w;
     }
 
@@ -305,10 +297,10 @@ struct KvWave {
             float top = x[y][0];
 #pragma unroll
             for (int j = 1; j < GK; ++j) top = fmaxf(top, x[y][j]);
-            if (__any(top > m[y] + (K::BIAS + K::SLACK))) {   // rare once the maximum is found: the reference moves, all sums with it
+            if (__any(top > m[y] + K::SLACK)) {   // rare once the maximum is found: the reference moves, all sums with it
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float mn = fmaxf(m[y], top - K::BIAS), c = __builtin_amdgcn_exp2f((m[y] - mn) * KV_LOG2E);
+                const float mn = fmaxf(m[y], top), c = __builtin_amdgcn_exp2f((m[y] - mn) * KV_LOG2E);
                 m[y] = mn;
                 l[y] *= c;
 #pragma unroll
@@ -335,10 +327,12 @@ struct KvWave {
 #pragma unroll
                     for (int y = 0; y < QT; ++y) o[y][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[j][i]), p[y][j], o[y][i], 0, 0, 0);
         } else {
-            // A weight is the sum of WP 16-bit numbers: with one alone a result is off by up to 2^-8 (bf16) where few keys share the weight, with
-            // two by less than 2^-16, which 16-bit results do not show; f32 results (over 8-bit pages) take three, all 24 bits.
-            // Values arrive as rows (key j: EV neighbouring columns a lane) and are needed as columns: pairs of rows are
-            // interleaved by byte permutes.
+            // With one bf16 number for a weight a result is off by up to 2^-8 where few keys share the weight, with two by 2^-17, which 16-bit
+            // results do not show; f32 results (over 8-bit pages) take three, all 24 bits.  f16 weights would spare the splitting of f16 values (32
+            // sequences of 1500, 20 heads of 64: 46.4 instead of 48.2 us; 447 keys of 8 heads: 6.0 instead of 6.9; 4000 keys of 32 values: 35
+            // instead of 42), but they lose bits from e^-12 of the largest weight on: a key's weight of e^-20 was off by 6 %.
+            // Values arrive as rows (key j: EV neighbouring columns a lane) and are needed as columns: 16-bit pairs of rows are
+            // interleaved by byte permutes, f16 ones as they are split.
             u4 weight[QT][K::WP];
 #pragma unroll
             for (int y = 0; y < QT; ++y)
@@ -358,15 +352,26 @@ struct KvWave {
                 }
 #pragma unroll
             for (int i = 0; i < EV; ++i) {
-                if constexpr (K::WP > 2) __builtin_amdgcn_sched_barrier(0);   // (columns in turn: registers for one more wave a SIMD; 128 short tables 12.8 -> 12.3 us)
-                u4 vt;
+                // (columns in turn: registers for one more wave a SIMD; 128 short tables of 8 bits, f32: 12.8 -> 12.3 us)
+                if constexpr (K::F16 || K::WP > 2) __builtin_amdgcn_sched_barrier(0);
+                u4 vt[K::VP];
 #pragma unroll
-                for (int jj = 0; jj < 4; ++jj)
-                    vt[jj] = __builtin_amdgcn_perm(w[2 * jj + 1][i / 2], w[2 * jj][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                for (int jj = 0; jj < 4; ++jj) {
+                    const uint32_t w0 = w[2 * jj][i / 2], w1 = w[2 * jj + 1][i / 2];
+                    if constexpr (K::F16) {
+                        float v0 = (float)__builtin_bit_cast(h2, w0)[i & 1], v1 = (float)__builtin_bit_cast(h2, w1)[i & 1];
 #pragma unroll
-                for (int n = K::WP - 1; n >= 0; --n)
+                        for (int n = 0; n < K::VP; ++n) vt[n][jj] = part(v0, v1);
+                    } else
+                        vt[0][jj] = __builtin_amdgcn_perm(w1, w0, i & 1 ? 0x07060302u : 0x05040100u);
+                }
 #pragma unroll
-                    for (int y = 0; y < QT; ++y) o[y][i] = mma(vt, weight[y][n], o[y][i]);
+                for (int n = K::WP + K::VP - 2; n >= 0; --n)   // the small products first; that of both last parts is 2^-18 of the largest
+#pragma unroll
+                    for (int h = 0; h < K::VP; ++h)
+                        if (n - h >= 0 && n - h < K::WP && !(h > 0 && n - h == K::WP - 1))
+#pragma unroll
+                            for (int y = 0; y < QT; ++y) o[y][i] = mma_bf16(vt[h], weight[y][n - h], o[y][i]);
             }
         }
     }
