@@ -19,6 +19,7 @@
  *  - The library keeps lazily-allocated device scratch arenas per (device,
  *    stream): per-unit reduction words, the banded mel filterbank, wt_kv_attend's
  *    workspace (17 MB with 256 compute units), and the DTW's direction bit planes (T*F/4 bytes per unit of the largest batch seen);
+ *    hipStreamPerThread is another stream, with arenas of its own, in every thread.
  *    wt_shutdown() frees them.  Growing an arena is a hipMalloc: warm a stream
  *    up once before capturing calls on it into a HIP graph.
  */
@@ -84,7 +85,7 @@ WT_API int wt_shutdown(void);
 /* Frees the scratch arenas the library keeps for `stream` on every device (the arenas are keyed by (device, purpose,
  * stream): a process that creates and destroys streams calls this before hipStreamDestroy, otherwise one arena set
  * per stream stays allocated until wt_shutdown).  The stream's queued work must have completed (the call does not
- * synchronise it).  Returns the number of arenas freed (>= 0). */
+ * synchronise it).  hipStreamPerThread: those of the calling thread.  Returns the number of arenas freed (>= 0). */
 WT_API int wt_release_stream(void *stream);
 
 /* T.py:783-793 hook_attention_weights.  Copies the LAST query row of n_sel heads of one decoder layer's

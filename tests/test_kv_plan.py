@@ -9,13 +9,13 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "whisper-timestamped_amd", "csrc")
 
 
-def host_program(folder, main):
+def host_program(folder, main, more=""):
     """The numbers that a host program over the header prints, line by line (nothing is launched)."""
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     if not os.path.exists(hipcc):
         pytest.skip("hipcc not found")
     src, exe = folder / "probe.hip", folder / "probe"
-    src.write_text('#include <cstdio>\n#include "wt_kv_plan.h"\nusing namespace wt;\nint main() {\n' + main + "\nreturn 0; }\n")
+    src.write_text('#include <cstdio>\n#include "wt_kv_plan.h"\n' + more + 'using namespace wt;\nint main() {\n' + main + "\nreturn 0; }\n")
     subprocess.check_call([hipcc, "--offload-arch=gfx950", "-std=c++17", "-I" + CSRC, "-I" + os.path.join(ROOT, "include"), str(src), "-o", str(exe)])
     return [tuple(map(int, line.split())) for line in subprocess.check_output([str(exe)], text=True).splitlines()]
 
@@ -40,3 +40,15 @@ def test_join_stays_in_its_workgroups_lds(tmp_path):
     assert all(far < 256 and led == 256 // lanes for *_, lanes, far, _, led in found)
     assert any(all_ >= 256 for *_, all_, _ in found), "the remainder that the rule is there for"
     assert (1, 32, 20, 3, 254, 257, 85) in found
+
+
+def test_a_threads_own_stream_has_memory_of_its_own(tmp_path):
+    """hipStreamPerThread is the same handle in every thread, and another stream: kept apart by thread; other handles are not."""
+    found = host_program(tmp_path, """
+        const hipStream_t other = reinterpret_cast<hipStream_t>(0x1000);
+        StreamKey mine = stream_key(hipStreamPerThread), theirs, theirs_other, next;
+        std::thread([&] { theirs = stream_key(hipStreamPerThread), theirs_other = stream_key(other); }).join();
+        std::thread([&] { next = stream_key(hipStreamPerThread); }).join();
+        std::printf("%d %d %d %d %d %d\\n", mine == stream_key(hipStreamPerThread), mine == theirs, theirs == next, mine == next,
+                    theirs_other == stream_key(other), stream_key(nullptr) == StreamKey{nullptr, 0});""", "#include <thread>\n#include \"wt_stream_key.h\"\n")
+    assert found == [(1, 0, 0, 0, 1, 1)]

@@ -8,6 +8,7 @@
 
 #include "wt_common.h"
 #include "wt_small.h"
+#include "wt_stream_key.h"
 
 namespace wt {
 
@@ -34,7 +35,7 @@ struct Arena {
 static std::mutex g_mu;
 // One arena per (device, purpose, stream): calls on distinct streams never share scratch (they may run concurrently),
 // calls on one stream are ordered by the stream.
-static std::map<std::tuple<int, int, hipStream_t>, Arena> g_arena;
+static std::map<std::tuple<int, int, StreamKey>, Arena> g_arena;
 
 // Growing is a hipMalloc (synchronising, not graph-capturable); the first call reserves at least 256 KB so that
 // steady state never grows.  `fresh` (optional) tells the caller that the memory is new (tags were reset).
@@ -42,7 +43,7 @@ static int scratch_ex(int purpose, hipStream_t st, size_t bytes, void **out, Are
     int dev = 0;
     WT_HIP(hipGetDevice(&dev));
     std::lock_guard<std::mutex> lk(g_mu);
-    Arena &a = g_arena[std::make_tuple(dev, purpose, st)];
+    Arena &a = g_arena[std::make_tuple(dev, purpose, stream_key(st))];
     if (bytes > a.cap) {
         size_t want = bytes < (256u << 10) ? (256u << 10) : bytes * 2;
         void *np = nullptr;
@@ -147,10 +148,11 @@ int wt_shutdown(void) {
 // set per stream until wt_shutdown.  The caller guarantees the stream's work has completed.
 int wt_release_stream(void *stream) {
     std::lock_guard<std::mutex> lk(wt::g_mu);
+    const wt::StreamKey mine = wt::stream_key((hipStream_t)stream);
     int freed = 0, cur = 0;
     (void)hipGetDevice(&cur);
     for (auto it = wt::g_arena.begin(); it != wt::g_arena.end();) {
-        if (std::get<2>(it->first) == (hipStream_t)stream) {
+        if (std::get<2>(it->first) == mine) {
             if (it->second.p) {
                 (void)hipSetDevice(std::get<0>(it->first));
                 (void)hipFree(it->second.p);
