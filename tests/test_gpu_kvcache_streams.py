@@ -52,3 +52,21 @@ def test_two_threads_on_their_own_streams():
     assert not bad
     for w, results in zip(want, outs):
         assert all(torch.equal(r, w) for r in results)
+
+
+def test_check_waits_for_every_stream():
+    """A call on another stream, still waiting behind other work, counts for check()."""
+    from whisper_timestamped._lib import WtError
+    cache, table, lens = long_cache(n=500)
+    q = torch.zeros((1, 2, 64), dtype=F16, device=DEV)
+    busy = torch.randn((4096, 4096), device=DEV)
+    bad = torch.tensor([table.shape[1] * 64 + 1], dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(30):
+            busy = busy @ busy * 1e-2
+        cache.attend(q, table, bad)
+    with pytest.raises(WtError, match="length"):
+        cache.check()
+    cache.check()

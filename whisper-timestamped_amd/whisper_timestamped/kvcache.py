@@ -94,10 +94,12 @@ class PagedKVCache:
         return self._calls.workspace(self._handle, table, n_q_heads)
 
     def check(self):
-        """Waits for the device; raises if a call since the last check met something outside of its range."""
+        """Waits for the device, all of its streams; raises if a call since the last check met something outside of its range."""
+        torch.cuda.synchronize(self.device)
         bits = int(self.error.item())
         if bits:
             self.error.zero_()
+            torch.cuda.synchronize(self.device)          # (cleared before a call on another stream can report again)
             said = {_lib.WT_KV_BAD_POSITION: "a position or length beyond the page table", _lib.WT_KV_BAD_PAGE: "a page outside of the cache",
                     _lib.WT_KV_BAD_SEQUENCE: "a sequence outside of the page table"}
             raise WtError("paged cache: " + ", ".join(s for b, s in said.items() if bits & b))
