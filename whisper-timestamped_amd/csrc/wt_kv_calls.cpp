@@ -15,6 +15,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include "wt_overlap.h"
 #include "wtalign.h"
 
 namespace {
@@ -31,7 +32,9 @@ struct Cache {
     int device;   // -1: host memory, whose every call is refused
     at::ScalarType type;
     at::Storage kept[5];   // what desc points into lives as long as it
+    wt::Strided3 memory[4];   // k, v and their exponents
 };
+constexpr const char *PARTS[4] = {"k", "v", "k_exp", "v_exp"};
 constexpr const char *CACHE = "wt_kv_cache";
 
 struct Refused {};   // the Python error is set
@@ -197,6 +200,13 @@ const at::Tensor &pages(PyObject *o, const char *name, int *dtype) {
     return t;
 }
 
+wt::Strided3 memory_of(const at::Tensor &t, int rows) {   // `rows` dimensions of rows of adjacent values
+    int64_t row = t.element_size(), stride[3];
+    for (int i = rows; i < t.dim(); ++i) row *= t.size(i);
+    for (int i = 0; i < rows; ++i) stride[i] = t.stride(i) * t.element_size();
+    return wt::Strided3(t.const_data_ptr(), row, rows, t.sizes().data(), stride);
+}
+
 // k, v, k_exp or None, v_exp or None, host (tensors of the host's memory are taken, for calls that are refused in the end) ->
 // (handle, error word)
 PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
@@ -210,6 +220,7 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
         if (k.const_data_ptr() == v.const_data_ptr()) refuse("k and v are the same memory");
         uint8_t *e[2] = {nullptr, nullptr};
         at::Storage es[2];
+        wt::Strided3 memory[4] = {memory_of(k, 3), memory_of(v, 3)};
         for (int i = 0; i < 2; ++i) {
             const char *name = i == 0 ? "k_exp" : "v_exp";
             if (is_none(args[2 + i]) == (dtype == WT_DTYPE_E4M3)) refuse("%s: a float8_e4m3fn cache has exponents, another has none", name);
@@ -221,8 +232,12 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
                 refuse("%s: contiguous uint8 (%ld, %ld, %ld) beside the pages, 16-byte aligned", name, (long)k.size(0), (long)k.size(1), (long)k.size(2));
             e[i] = static_cast<uint8_t *>(x.data_ptr());
             es[i] = x.storage();
+            memory[2 + i] = memory_of(x, 0);
         }
         if (e[0] && e[0] == e[1]) refuse("k_exp and v_exp are the same memory");
+        for (int i = 0; i < 4; ++i)
+            for (int j = i + 1; j < 4; ++j)
+                if (k.device() == v.device() && wt::overlap(memory[i], memory[j])) refuse("%s and %s share memory", PARTS[i], PARTS[j]);
         const int host = PyObject_IsTrue(args[4]);
         if (host < 0) return nullptr;
         if (!k.is_cuda() && !(host && k.is_cpu())) refuse("k must be on the GPU: the cache's kernels only run there");
@@ -233,7 +248,8 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
                               (int32_t)k.size(0), (int32_t)k.size(1), (int32_t)k.size(2), (int32_t)k.size(3), dtype, 0, error.data_ptr<int32_t>()},
                              k.is_cuda() ? (int)k.get_device() : -1,
                              k.scalar_type(),
-                             {k.storage(), v.storage(), es[0], es[1], error.storage()}};
+                             {k.storage(), v.storage(), es[0], es[1], error.storage()},
+                             {memory[0], memory[1], memory[2], memory[3]}};
         PyObject *handle = PyCapsule_New(c, CACHE, [](PyObject *o) { delete static_cast<Cache *>(PyCapsule_GetPointer(o, CACHE)); });
         if (!handle) {
             delete c;
