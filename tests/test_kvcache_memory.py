@@ -7,7 +7,7 @@ import subprocess
 import pytest
 import torch
 
-from test_kvcache_host import E4M3, pages
+from test_kvcache_host import E4M3, TABLE, i32, pages
 from whisper_timestamped import PagedKVCache
 from whisper_timestamped._lib import WtError
 
@@ -94,3 +94,36 @@ def test_exponents_share_nothing():
         PagedKVCache(k, v, inside, two)
     with pytest.raises(WtError, match="GPU"):
         PagedKVCache(k, v, one, e[128:256].view(4, 2, 16))
+
+
+def cache_over(k, v, *e):
+    from whisper_timestamped import kvcache
+    cache = object.__new__(PagedKVCache)
+    cache._calls = kvcache._calls()
+    cache._handle, cache.error = cache._calls.make(k, v, *(e or (None, None)), True)
+    return cache
+
+
+def test_rows_are_not_the_caches_own_memory():
+    """append reads rows while it writes the cache, gather and attend write results while they read it."""
+    mem = torch.zeros(3, *SHAPE, dtype=torch.float16)
+    cache = cache_over(mem[0], mem[1])
+    free = mem[2].reshape(-1)[:3 * 2 * 64].view(3, 2, 64)
+    own = [m.reshape(-1)[256:256 + 3 * 2 * 64].view(3, 2, 64) for m in mem[:2]]
+    pos = i32(0, 1, 2)
+    for mine in own:
+        for k, v, name in ((mine, free, "k"), (free, mine, "v")):
+            with pytest.raises(WtError, match=f"{name}: the cache's own memory"):
+                cache.append(k, v, TABLE, pos)
+            with pytest.raises(WtError, match=r"out\[%d\]: the cache's own memory" % (name == "v")):
+                cache.gather(TABLE, pos, out=(k, v.clone()) if name == "k" else (k.clone(), v))
+        with pytest.raises(WtError, match="out: the cache's own memory"):
+            cache.attend(free, TABLE, pos, out=mine)
+    with pytest.raises(WtError, match="only run on the GPU"):
+        cache.append(free, free, TABLE, pos)                      # (beside the cache in one piece of memory: fine)
+    e = [torch.zeros(4, 2, 16, dtype=torch.uint8) for _ in range(2)]
+    cache = cache_over(pages(*SHAPE, dtype=E4M3), pages(*SHAPE, dtype=E4M3), *e)
+    wide = pages(3, 2, 64)
+    rows = e[1].reshape(-1).view(torch.float16).as_strided((3, 2, 64), (0, 0, 1))
+    with pytest.raises(WtError, match="k: the cache's own memory"):
+        cache.append(rows, wide, TABLE, pos)

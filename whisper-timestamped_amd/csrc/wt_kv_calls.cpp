@@ -129,6 +129,18 @@ Strided strided(const at::Tensor &t, const Cache *c, const char *name, int64_t n
     return s;
 }
 
+wt::Strided3 memory_of(const at::Tensor &t, int rows) {   // `rows` dimensions of rows of adjacent values
+    int64_t row = t.element_size(), stride[3];
+    for (int i = rows; i < t.dim(); ++i) row *= t.size(i);
+    for (int i = 0; i < rows; ++i) stride[i] = t.stride(i) * t.element_size();
+    return wt::Strided3(t.const_data_ptr(), row, rows, t.sizes().data(), stride);
+}
+
+void not_the_caches(const wt::Strided3 &m, const Cache *c, const char *name) {
+    for (const wt::Strided3 &part : c->memory)
+        if (wt::overlap(m, part)) refuse("%s: the cache's own memory", name);
+}
+
 // the cache's device is the current one, and its current stream the launch's
 struct On {
     int before = -1;
@@ -198,13 +210,6 @@ const at::Tensor &pages(PyObject *o, const char *name, int *dtype) {
         extent += t.stride(order[i]) * (t.size(order[i]) - 1);
     }
     return t;
-}
-
-wt::Strided3 memory_of(const at::Tensor &t, int rows) {   // `rows` dimensions of rows of adjacent values
-    int64_t row = t.element_size(), stride[3];
-    for (int i = rows; i < t.dim(); ++i) row *= t.size(i);
-    for (int i = 0; i < rows; ++i) stride[i] = t.stride(i) * t.element_size();
-    return wt::Strided3(t.const_data_ptr(), row, rows, t.sizes().data(), stride);
 }
 
 // k, v, k_exp or None, v_exp or None, host (tensors of the host's memory are taken, for calls that are refused in the end) ->
@@ -281,6 +286,7 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n) {
         no_gradient(k, "k"), no_gradient(v, "v");
         const int dt = dtype_of(k.scalar_type(), c, "k, v");
         const Strided ks = strided(k, c, "k", r.n, c->desc.n_heads, true), vs = strided(v, c, "v", r.n, c->desc.n_heads, true);
+        not_the_caches(memory_of(k, 2), c, "k"), not_the_caches(memory_of(v, 2), c, "v");
         if (r.n > 0) {
             const On on(c);
             check(g_append(&c->desc, ks.p, vs.p, dt, ks.row, ks.head, vs.row, vs.head, r.n, r.table.p, r.table.stride, r.table.n, r.table.width,
@@ -316,6 +322,7 @@ PyObject *gather(PyObject *, PyObject *const *args, Py_ssize_t n) {
             no_gradient(k, "out[0]"), no_gradient(v, "out[1]");
             strided(k, c, "out[0]", r.n, c->desc.n_heads, true), strided(v, c, "out[1]", r.n, c->desc.n_heads, true);
             if (!k.is_contiguous() || !v.is_contiguous()) refuse("out: not contiguous");
+            not_the_caches(memory_of(k, 0), c, "out[0]"), not_the_caches(memory_of(v, 0), c, "out[1]");
             const char *kp = static_cast<const char *>(k.const_data_ptr()), *vp = static_cast<const char *>(v.const_data_ptr());
             if (r.n > 0 && kp < vp + v.nbytes() && vp < kp + k.nbytes()) refuse("out: the same memory twice");
         }
@@ -417,6 +424,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
             const bool rows_outside = os.head >= d && os.row >= (heads - 1) * os.head + d, heads_outside = os.row >= d && os.head >= (t.n - 1) * os.row + d;
             if (t.n > 1 && heads > 1 ? !rows_outside && !heads_outside : (t.n > 1 && os.row < d) || (heads > 1 && os.head < d))
                 refuse("out: two heads' values in one place (strides %ld, %ld)", (long)os.row, (long)os.head);
+            not_the_caches(memory_of(out, 2), c, "out");
         }
         if (c->device < 0) refuse("the cache's kernels only run on the GPU");
         if (!out.defined()) {
