@@ -352,7 +352,7 @@ WT_API int wt_kv_gather(const wt_kv_cache *cache, void *k, void *v, int dtype, i
  * that do take part leaves its element infinite or NaN.  Sums of values run up to exp(8) * sum |v_t| before they are divided: where
  * that is beyond 2^128 the result is not finite, and of values below 2^-100 bits are lost.
  *   q, out : device, dtype F32 / F16 / BF16 (the cache's own; any of them over an E4M3 cache), head_dim values in a row;
- *            out may be q.  Rows beyond n_seqs are not touched
+ *            out may be q, and shares no memory with it otherwise.  Rows beyond n_seqs are not touched
  *   lse    : optional device fp32 [n_seqs][n_q_heads]
  *   workspace : wt_kv_attend_workspace() bytes of device memory, 16-byte aligned, its first WT_KV_WORKSPACE_ZEROED bytes zeroed
  *            once before its first use; every call leaves it ready for the next one.  Two calls that may run at the same time (on two streams, or in two

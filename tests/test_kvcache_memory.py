@@ -7,7 +7,7 @@ import subprocess
 import pytest
 import torch
 
-from test_kvcache_host import E4M3, TABLE, i32, pages
+from test_kvcache_host import E4M3, TABLE, host_cache, i32, pages
 from whisper_timestamped import PagedKVCache
 from whisper_timestamped._lib import WtError
 
@@ -127,3 +127,18 @@ def test_rows_are_not_the_caches_own_memory():
     rows = e[1].reshape(-1).view(torch.float16).as_strided((3, 2, 64), (0, 0, 1))
     with pytest.raises(WtError, match="k: the cache's own memory"):
         cache.append(rows, wide, TABLE, pos)
+
+
+def test_results_and_queries():
+    """out is q itself, or shares nothing with it: side by side in one tensor is fine, a few values or rows apart is not."""
+    base = torch.zeros(4000, dtype=torch.float16)
+    q = base.as_strided((3, 4, 64), (512, 64, 1), 0)
+    for out, said in ((q, "GPU"), (base.as_strided((3, 4, 64), (512, 64, 1), 256), "GPU"), (base.as_strided((3, 4, 64), (512, 64, 1), 255), "out: shares memory"),
+                      (base.as_strided((3, 4, 64), (512, 64, 1), 64), "out: shares memory"), (base.as_strided((3, 4, 64), (512, 64, 1), 512), "out: shares memory"),
+                      (base.as_strided((3, 4, 64), (256, 64, 1), 0), "out: shares memory"), (base.as_strided((3, 4, 64), (256, 64, 1), 1536), "GPU")):
+        with pytest.raises(WtError, match=said):
+            host_cache().attend(q, TABLE, i32(1, 2, 3), out=out)
+    # one query for two sequences and the results of both: the first one's result is where the second still reads
+    both = torch.zeros(512, dtype=torch.float16)
+    with pytest.raises(WtError, match="out: shares memory"):
+        host_cache().attend(both.as_strided((2, 4, 64), (0, 64, 1)), TABLE[:2], i32(1, 2), out=both.view(2, 4, 64))

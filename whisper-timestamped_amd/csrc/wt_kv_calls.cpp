@@ -424,7 +424,10 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
             const bool rows_outside = os.head >= d && os.row >= (heads - 1) * os.head + d, heads_outside = os.row >= d && os.head >= (t.n - 1) * os.row + d;
             if (t.n > 1 && heads > 1 ? !rows_outside && !heads_outside : (t.n > 1 && os.row < d) || (heads > 1 && os.head < d))
                 refuse("out: two heads' values in one place (strides %ld, %ld)", (long)os.row, (long)os.head);
-            not_the_caches(memory_of(out, 2), c, "out");
+            const wt::Strided3 result = memory_of(out, 2), query = memory_of(q, 2);
+            not_the_caches(result, c, "out");
+            if (!(qs.p == os.p && qs.row == os.row && qs.head == os.head) && wt::overlap(result, query))   // (a row's query is read before its result is written)
+                refuse("out: shares memory with q without being q");
         }
         if (c->device < 0) refuse("the cache's kernels only run on the GPU");
         if (!out.defined()) {

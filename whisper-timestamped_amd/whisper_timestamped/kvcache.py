@@ -80,7 +80,7 @@ class PagedKVCache:
         """One new token of every sequence: q (B, query heads, head_dim) over the sequence's positions 0 ... lengths[b] - 1;
         query head h reads key head h // (query heads // heads).  -> (B, query heads, head_dim) in q's type, with
         ``return_lse`` also the float32 (B, query heads) logarithm of its sum of exponentials.  A length of zero gives
-        zeros (and -inf).  ``scale``: default head_dim ** -0.5.  ``out`` may be q itself.
+        zeros (and -inf).  ``scale``: default head_dim ** -0.5.  ``out`` may be q itself, and shares no memory with it otherwise.
 
         Long sequences are split over workgroups that meet in a workspace: the library's own of the current stream, or
         ``workspace`` (from ``attend_workspace``).  Calls that may run at the same time need one each.  A call that is being
