@@ -10,6 +10,7 @@
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -53,12 +54,19 @@ Cache *cache_of(PyObject *o) {
     if (!c) throw Refused();
     return c;
 }
+// A tensor that means what its memory holds and nothing else
+void plain(const at::Tensor &t, const char *name) {
+    if (t.is_neg()) refuse("%s: a view that is negated when it is read: call resolve_neg()", name);
+    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        refuse("%s has a tangent (forward-mode differentiation), which the cache's calls do not have", name);
+}
 const at::Tensor &tensor(PyObject *o, const Cache *c, const char *name, int64_t dim) {
     if (!THPVariable_Check(o)) refuse("%s: not a tensor", name);
     const at::Tensor &t = THPVariable_Unpack(o);
     if (t.layout() != at::kStrided || (t.is_cuda() ? (int)t.get_device() : t.is_cpu() ? -1 : -2) != c->device)
         refuse("%s: not a tensor of the cache's device", name);
     if (t.dim() != dim) refuse("%s: %d dimensions, not %d", name, (int)t.dim(), (int)dim);
+    plain(t, name);
     return t;
 }
 bool is_none(PyObject *o) { return o == Py_None; }
@@ -189,6 +197,7 @@ const at::Tensor &pages(PyObject *o, const char *name, int *dtype) {
     *dtype = s == at::kFloat ? WT_DTYPE_F32 : s == at::kHalf ? WT_DTYPE_F16 : s == at::kBFloat16 ? WT_DTYPE_BF16 : s == at::kFloat8_e4m3fn ? WT_DTYPE_E4M3 : -1;
     if (t.layout() != at::kStrided || t.dim() != 4 || *dtype < 0)
         refuse("%s: a 4-dimensional tensor (pages, heads, slots, head_dim) of float32, float16, bfloat16 or float8_e4m3fn", name);
+    plain(t, name);
     const int64_t d = t.size(3);
     if (t.numel() == 0 || (d != 32 && d != 64 && d != 96 && d != 128 && d != 256))
         refuse("%s: (%ld, %ld, %ld, %ld); head_dim is 32, 64, 96, 128 or 256, nothing is empty", name, (long)t.size(0), (long)t.size(1), (long)t.size(2), (long)d);
