@@ -33,6 +33,8 @@ struct Cache {
     int device;   // -1: host memory, whose every call is refused
     at::ScalarType type;
     at::Storage kept[5];   // what desc points into lives as long as it
+    const void *start[5];  // ... and has to be where it was
+    size_t bytes[5];
     wt::Strided3 memory[4];   // k, v and their exponents
 };
 constexpr const char *PARTS[4] = {"k", "v", "k_exp", "v_exp"};
@@ -52,10 +54,19 @@ void check(int64_t rc, const char *what) {
 Cache *cache_of(PyObject *o) {
     Cache *c = static_cast<Cache *>(PyCapsule_GetPointer(o, CACHE));
     if (!c) throw Refused();
+    for (int i = 0; i < 5; ++i)
+        if (c->kept[i] && (c->kept[i].data() != c->start[i] || c->kept[i].nbytes() < c->bytes[i]))
+            refuse("the cache's memory has been resized or moved since it was made");
     return c;
 }
-// A tensor that means what its memory holds and nothing else
+// A tensor that means what its memory holds and nothing else, and whose memory is there: a storage may have been resized under it
 void plain(const at::Tensor &t, const char *name) {
+    if (t.numel() > 0) {
+        int64_t last = t.storage_offset();
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        if (!t.has_storage() || !t.storage().data() || (uint64_t)(last + 1) * t.element_size() > t.storage().nbytes())
+            refuse("%s: not all of it has memory", name);
+    }
     if (t.is_neg()) refuse("%s: a view that is negated when it is read: call resolve_neg()", name);
     if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
         refuse("%s has a tangent (forward-mode differentiation), which the cache's calls do not have", name);
@@ -241,9 +252,10 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
             if (dtype != WT_DTYPE_E4M3) continue;
             if (!THPVariable_Check(args[2 + i])) refuse("%s: not a tensor", name);
             const at::Tensor &x = THPVariable_Unpack(args[2 + i]);
-            if (x.scalar_type() != at::kByte || x.dim() != 3 || x.size(0) != k.size(0) || x.size(1) != k.size(1) || x.size(2) != k.size(2) ||
+            if (x.layout() != at::kStrided || x.scalar_type() != at::kByte || x.dim() != 3 || x.size(0) != k.size(0) || x.size(1) != k.size(1) || x.size(2) != k.size(2) ||
                 !x.is_contiguous() || ((uintptr_t)x.const_data_ptr() & 15) || x.device() != k.device())
                 refuse("%s: contiguous uint8 (%ld, %ld, %ld) beside the pages, 16-byte aligned", name, (long)k.size(0), (long)k.size(1), (long)k.size(2));
+            plain(x, name);
             e[i] = static_cast<uint8_t *>(x.data_ptr());
             es[i] = x.storage();
             memory[2 + i] = memory_of(x, 0);
@@ -263,7 +275,11 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
                              k.is_cuda() ? (int)k.get_device() : -1,
                              k.scalar_type(),
                              {k.storage(), v.storage(), es[0], es[1], error.storage()},
+                             {},
+                             {},
                              {memory[0], memory[1], memory[2], memory[3]}};
+        for (int i = 0; i < 5; ++i)
+            if (c->kept[i]) c->start[i] = c->kept[i].data(), c->bytes[i] = c->kept[i].nbytes();
         PyObject *handle = PyCapsule_New(c, CACHE, [](PyObject *o) { delete static_cast<Cache *>(PyCapsule_GetPointer(o, CACHE)); });
         if (!handle) {
             delete c;
