@@ -36,6 +36,7 @@ struct Cache {
     const void *start[5];  // ... and has to be where it was
     size_t bytes[5];
     wt::Strided3 memory[4];   // k, v and their exponents
+    c10::VariableVersion version[4];
 };
 constexpr const char *PARTS[4] = {"k", "v", "k_exp", "v_exp"};
 constexpr const char *CACHE = "wt_kv_cache";
@@ -81,6 +82,12 @@ const at::Tensor &tensor(PyObject *o, const Cache *c, const char *name, int64_t 
     return t;
 }
 bool is_none(PyObject *o) { return o == Py_None; }
+
+// what a call has written: autograd's saved tensors in the same memory are out of date (inference tensors have no versions)
+void written(c10::VariableVersion version) {
+    if (version.enabled()) version.bump();
+}
+c10::VariableVersion version_of(const at::Tensor &t) { return t.unsafeGetTensorImpl()->version_counter(); }
 
 // Nothing here has a gradient; a call that autograd would have to record is refused rather than left out of the graph.
 void no_gradient(const at::Tensor &t, const char *name) {
@@ -246,6 +253,7 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
         uint8_t *e[2] = {nullptr, nullptr};
         at::Storage es[2];
         wt::Strided3 memory[4] = {memory_of(k, 3), memory_of(v, 3)};
+        c10::VariableVersion version[4] = {version_of(k), version_of(v), version_of(k), version_of(v)};
         for (int i = 0; i < 2; ++i) {
             const char *name = i == 0 ? "k_exp" : "v_exp";
             if (is_none(args[2 + i]) == (dtype == WT_DTYPE_E4M3)) refuse("%s: a float8_e4m3fn cache has exponents, another has none", name);
@@ -259,6 +267,7 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
             e[i] = static_cast<uint8_t *>(x.data_ptr());
             es[i] = x.storage();
             memory[2 + i] = memory_of(x, 0);
+            version[2 + i] = version_of(x);
         }
         if (e[0] && e[0] == e[1]) refuse("k_exp and v_exp are the same memory");
         for (int i = 0; i < 4; ++i)
@@ -277,7 +286,8 @@ PyObject *make(PyObject *, PyObject *const *args, Py_ssize_t n) {
                              {k.storage(), v.storage(), es[0], es[1], error.storage()},
                              {},
                              {},
-                             {memory[0], memory[1], memory[2], memory[3]}};
+                             {memory[0], memory[1], memory[2], memory[3]},
+                             {version[0], version[1], version[2], version[3]}};
         for (int i = 0; i < 5; ++i)
             if (c->kept[i]) c->start[i] = c->kept[i].data(), c->bytes[i] = c->kept[i].nbytes();
         PyObject *handle = PyCapsule_New(c, CACHE, [](PyObject *o) { delete static_cast<Cache *>(PyCapsule_GetPointer(o, CACHE)); });
@@ -317,6 +327,7 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n) {
             check(g_append(&c->desc, ks.p, vs.p, dt, ks.row, ks.head, vs.row, vs.head, r.n, r.table.p, r.table.stride, r.table.n, r.table.width,
                            r.sequences, r.positions, on.stream),
                   "wt_kv_append");
+            for (int i = 0; i < (c->desc.dtype == WT_DTYPE_E4M3 ? 4 : 2); ++i) written(c->version[i]);
         }
         Py_RETURN_NONE;
     } catch (const Refused &) {
@@ -363,6 +374,7 @@ PyObject *gather(PyObject *, PyObject *const *args, Py_ssize_t n) {
             check(g_gather(&c->desc, k.data_ptr(), v.data_ptr(), dt, r.n, r.table.p, r.table.stride, r.table.n, r.table.width, r.sequences,
                            r.positions, on.stream),
                   "wt_kv_gather");
+            written(version_of(k)), written(version_of(v));
         }
         if (!is_none(args[5])) {
             Py_INCREF(args[5]);
@@ -473,6 +485,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
                 rc = go();
             }
             check(rc, "wt_kv_attend");
+            written(version_of(out));
         }
         PyObject *o;
         if (is_none(args[5])) o = THPVariable_Wrap(out);
