@@ -33,6 +33,7 @@ EXPORTS = ["wt_version", "wt_last_error", "wt_shutdown", "wt_cost_batch", "wt_dt
            "wt_disfluency_batch", "wt_qk_rows_batch", "wt_logprob_gather_rows", "wt_dtw_batch_pattern", "wt_align_batch_v3",
            "wt_release_stream", "wt_qk_rows_streams", "wt_logmel_pad_batch", "wt_logprob_digest_streams",
            "wt_kv_append", "wt_kv_gather", "wt_kv_attend", "wt_kv_attend_workspace"]
+KV_EXPORTS = EXPORTS[-4:]                                    # the paged cache's (kvcache.py): a library without them serves the rest
 WT_STEP_SYMMETRIC1, WT_STEP_NO_EMPTY_SUBWORDS = 0, 1
 ABI_VERSION = 5
 WT_KV_BAD_POSITION, WT_KV_BAD_PAGE, WT_KV_BAD_SEQUENCE = 1, 2, 4
@@ -66,6 +67,9 @@ def load():
         raise ImportError(f"{LIB_PATH} is missing: build it with `make -C {_PKG_ROOT}/csrc` "
                           "(or __graft_entry__.build()); there is no CPU fallback")
     L = ctypes.CDLL(LIB_PATH)
+    missing = [n for n in EXPORTS if not hasattr(L, n)]      # (entries may be added within an ABI version)
+    if set(missing) - set(KV_EXPORTS):
+        raise ImportError(f"{LIB_PATH} lacks {', '.join(missing)}: rebuild it (`make -C {_PKG_ROOT}/csrc`)")
     vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
     L.wt_version.restype = i32
     L.wt_last_error.restype = ctypes.c_char_p
@@ -89,19 +93,19 @@ def load():
     L.wt_qk_rows_streams.argtypes = [vp, vp, i32, i32, i32, i32, i64, i64, i32, i32, i32, f32, vp, vp, vp, i32, vp, vp, i32, i64,
                                      i64, i64, vp]
     L.wt_logprob_digest_streams.argtypes = [vp, i64, i32, i32, vp, i32, i64, vp, i64, i64, vp, i32, i32, vp, vp, vp]
-    missing = [n for n in EXPORTS if not hasattr(L, n)]      # (entries may be added within an ABI version)
-    if missing:
-        raise ImportError(f"{LIB_PATH} lacks {', '.join(missing)}: rebuild it (`make -C {_PKG_ROOT}/csrc`)")
-    L.wt_kv_append.argtypes = [vp, vp, vp, i32, i64, i64, i64, i64, i32, vp, i64, i32, i32, vp, vp, vp]
-    L.wt_kv_gather.argtypes = [vp, vp, vp, i32, i32, vp, i64, i32, i32, vp, vp, vp]
-    L.wt_kv_attend.argtypes = [vp, vp, i32, i64, i64, i32, i32, f32, vp, i64, i32, vp, vp, i64, i64, vp, vp, i64, vp]
-    L.wt_kv_attend_workspace.argtypes = [vp, i32, i32, i32]
+    if not missing:
+        L.wt_kv_append.argtypes = [vp, vp, vp, i32, i64, i64, i64, i64, i32, vp, i64, i32, i32, vp, vp, vp]
+        L.wt_kv_gather.argtypes = [vp, vp, vp, i32, i32, vp, i64, i32, i32, vp, vp, vp]
+        L.wt_kv_attend.argtypes = [vp, vp, i32, i64, i64, i32, i32, f32, vp, i64, i32, vp, vp, i64, i64, vp, vp, i64, vp]
+        L.wt_kv_attend_workspace.argtypes = [vp, i32, i32, i32]
     if L.wt_version() != ABI_VERSION:
         raise ImportError(f"{LIB_PATH} exports ABI version {L.wt_version()}, this package needs {ABI_VERSION}: rebuild it "
                           f"(`make -C {_PKG_ROOT}/csrc`)")
     for n in EXPORTS[3:]:
-        getattr(L, n).restype = i32
-    L.wt_kv_attend_workspace.restype = i64
+        if n not in missing:
+            getattr(L, n).restype = i32
+    if not missing:
+        L.wt_kv_attend_workspace.restype = i64
     _lib = L
     return L
 

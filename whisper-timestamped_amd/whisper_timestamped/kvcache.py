@@ -33,6 +33,9 @@ HEAD_DIMS = (32, 64, 96, 128, 256)
 def _calls():
     """The module of the calls, on the entries of the library that ``_lib`` has loaded."""
     L = _lib.load()
+    missing = [n for n in _lib.KV_EXPORTS if not hasattr(L, n)]
+    if missing:
+        raise ImportError(f"{_lib.LIB_PATH} lacks {', '.join(missing)}: rebuild it (`make -C {_lib._PKG_ROOT}/csrc`)")
     try:
         from . import _kvcalls
     except ImportError as err:
