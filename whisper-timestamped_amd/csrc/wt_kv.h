@@ -97,12 +97,6 @@ struct alignas((sizeof(T) * N & -(sizeof(T) * N)) > 16 ? 16 : sizeof(T) * N & -(
 static_assert(sizeof(Pack<float, 6>) == 24 && sizeof(Pack<uint16_t, 6>) == 12 && sizeof(Pack<uint16_t, 8>) == 16, "no padding");
 
 
-constexpr int KV_WAVES = 4;   // waves of a workgroup of the attention kernel
-
-constexpr int KV_WIDE_HD = 128;   // widest heads whose queries may be taken 32 at a time (beyond, registers run out)
-
-constexpr int kv_slot(int head_dim, int q_wide) { return q_wide * (64 + 16 * head_dim); }   // floats of a partial result
-
 // arguments of one attention call, as its kernels take them (wt_kv_attend.h)
 struct KvAttend {
     KvRows k, v;
