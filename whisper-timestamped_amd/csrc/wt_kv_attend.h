@@ -692,8 +692,8 @@ __device__ __forceinline__ void kv_join(const KvAttend &a, float *lds, int s, in
 }
 
 // Short tables: one workgroup per (sequence, key head, query tile).  One head is bound by what a compute unit streams and by the
-// chain length -> table -> keys -> joining waves (447 keys of 8 heads, f16, 64 values: 6.3 us), many by memory (32 sequences of 1500, 20
-// heads: 45 us, 5.4 TB/s).
+// chain length -> table -> keys -> joining waves (447 keys of 8 heads, f16, 64 values: 7.1 us), many by memory (32 sequences of 1500, 20
+// heads: 47 us, 5.2 TB/s).
 template <typename CT, typename T, int HD, int PG, int NW, int QT>
 __global__ __launch_bounds__(NW * 64, HD * QT <= 128 ? 2 : 1) void kv_attend_direct_kernel(const KvAttend a) {
     extern __shared__ __attribute__((aligned(16))) float kv_lds[];

@@ -10,7 +10,7 @@ once, nothing that is there moves, and the pages may hold 8-bit codes with one p
     out = cache.attend(q, table, lengths)         # (B, 8, 64): each over its own positions 0 ... lengths[b] - 1
     k_rows, v_rows = cache.gather(table, positions, sequences=seq)
 
-``table`` (int32, (B, width)): row b lists the pages of sequence b in order; entries behind its last page are never read.
+``table`` (int32, (B, width)): row b lists the pages of sequence b in order; entries behind its last page may be read, but are never followed.
 Everything runs on the current stream of the cache's device and reads tables, positions and lengths on the device: a
 captured graph follows them from replay to replay.  ``check()`` (which waits for the device) raises if a call since the
 last check met a sequence, position, length or page outside of its range; such a call reads and writes nothing there
