@@ -125,3 +125,13 @@ def test_known_results_tell_a_lost_key():
         for p in [p for p in range(n) if int(at[p]) in columns.tolist()][::97]:
             wrong, _ = K.peak_results(x, at, n, columns, s.q_dtype, s.depth(), without=p // K.RUN * K.RUN)
             assert float(((wrong - want).abs() / allowed).max()) > 2.0, (s, p)
+
+
+def test_very_many_heads_over_very_long_tables(tmp_path):
+    """2^27 heads over tables of 2^40 bytes are more than 64 MB, although their product has no place in 64 bits."""
+    found = host_program(tmp_path, PLAN + """
+        for (int seqs : {1 << 10, 1 << 17, 1 << 22}) {
+            const KvPlan p = plan(256, WT_DTYPE_BF16, 128, 1 << 20, 32, seqs, 32 * 24, 2047);
+            std::printf("%d %d %d\\n", p.direct, p.q_wide, p.grid == 256);
+        }""")
+    assert found == [(0, 2, 1)] * 3

@@ -62,7 +62,7 @@ inline KvPlan kv_plan(int cus, const wt_kv_cache &c, int n_seqs, int n_q_heads, 
     // values 39 / 27 ... 179 / 106, 128 values 81 / 76 ... 402 / 238.  Shares, tables of 50, 100 and 300 (8 bits) or 600 MB in all: bf16, 128 values
     // 24.0 / 26.3, 41.5 / 33.6, 193 / 109, f16, 64 values 23.9 / 21.9, 39.8 / 31.1, 192 / 110, 8 bits, 128 values 28.0 / 28.5, 42.6 / 40.5, 106 / 73.
     const bool widen = is_direct(narrow) ? narrow > n && (c.head_dim <= 64 || c.dtype == WT_DTYPE_F32 || capacity >= 128 * 1024)
-                                         : heads * capacity >= 64 * 1024 * 1024;
+                                         : (double)heads * (double)capacity >= 64. * 1024 * 1024;
     p.q_wide = group > 16 && c.head_dim <= KV_WIDE_HD && widen ? 2 : 1;
     p.q_tiles = (group + 16 * p.q_wide - 1) / (16 * p.q_wide);
     const int64_t pairs = heads * p.q_tiles;
