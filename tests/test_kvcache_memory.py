@@ -142,3 +142,16 @@ def test_results_and_queries():
     both = torch.zeros(512, dtype=torch.float16)
     with pytest.raises(WtError, match="out: shares memory"):
         host_cache().attend(both.as_strided((2, 4, 64), (0, 64, 1)), TABLE[:2], i32(1, 2), out=both.view(2, 4, 64))
+
+
+def test_lazy_clones_are_pieces_of_their_own():
+    """Two lazy clones of one tensor share its memory until one is written: they are two tensors, and what they came from is a third."""
+    base = pages(*SHAPE)
+    k, v = base._lazy_clone(), base._lazy_clone()
+    cache = cache_over(k, v)
+    rows = base.reshape(-1)[:3 * 2 * 64].view(3, 2, 64)
+    with pytest.raises(WtError, match="only run on the GPU"):
+        cache.append(rows, rows, TABLE, i32(0, 1, 2))
+    mine = k.reshape(-1)[:3 * 2 * 64].view(3, 2, 64)
+    with pytest.raises(WtError, match="k: the cache's own memory"):
+        cache.append(mine, rows, TABLE, i32(0, 1, 2))

@@ -216,6 +216,7 @@ const at::Tensor &pages(PyObject *o, const char *name, int *dtype) {
     if (t.layout() != at::kStrided || t.dim() != 4 || *dtype < 0)
         refuse("%s: a 4-dimensional tensor (pages, heads, slots, head_dim) of float32, float16, bfloat16 or float8_e4m3fn", name);
     plain(t, name);
+    t.mutable_data_ptr();   // (a lazy clone gets its memory now, before addresses are compared and kept)
     const int64_t d = t.size(3);
     if (t.numel() == 0 || (d != 32 && d != 64 && d != 96 && d != 128 && d != 256))
         refuse("%s: (%ld, %ld, %ld, %ld); head_dim is 32, 64, 96, 128 or 256, nothing is empty", name, (long)t.size(0), (long)t.size(1), (long)t.size(2), (long)d);
