@@ -70,3 +70,35 @@ def test_check_waits_for_every_stream():
     with pytest.raises(WtError, match="length"):
         cache.check()
     cache.check()
+
+
+@pytest.mark.parametrize("width,group,columns", [(256, 16, None), (128, 32, 2100), (32, 24, None)])
+@pytest.mark.parametrize("given", [False, True])
+def test_captured_calls_with_much_shared_memory(width, group, columns, given):
+    """16 queries of 256 values and 32 of 128 need more LDS than a launch gets unasked, and split tables a workspace: captured, replayed
+    several times with other queries and lengths and with eager calls between, each replay as the eager call."""
+    cache, table, _ = long_cache(n=9000, heads=1, width=width, dtype=BF16)
+    if columns:
+        table = torch.cat([table, torch.full((1, columns - table.shape[1]), -7, dtype=torch.int32, device=DEV)], 1)
+    q, out = torch.zeros((1, group, width), dtype=BF16, device=DEV), torch.zeros((1, group, width), dtype=BF16, device=DEV)
+    lens = torch.tensor([9000], dtype=torch.int32, device=DEV)
+    ws = cache.attend_workspace(group, table)
+    assert ws is not None
+    cache.attend(q, table, lens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attend(q, table, lens, out=out, workspace=ws if given else None)
+    for turn, n in enumerate((9000, 1, 0, 4321, 9000)):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(turn)))
+        lens.fill_(n)
+        want = cache.attend(q, table, lens)
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), n
+        graph.replay()
+        again = cache.attend(q, table, lens)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(again, want), n
+    cache.check()
