@@ -293,6 +293,7 @@ WT_API int wt_logmel_pad_batch(const float *pcm, int n_chunks, int64_t n_samples
  * sequence s lives in page table[s * table_stride + p / page_size], slot p % page_size; element d of head h of a key at
  *     k[page * k_page_stride + h * k_head_stride + slot * k_slot_stride + d]                       (strides in elements)
  * so (page, head, slot) may be laid out in any order.  Base addresses and strides are multiples of 16 bytes.
+ * Keys, values and exponents share no byte with each other, nor with the rows and results of a call.
  *   dtype F32 / F16 / BF16: the values as they are.
  *   dtype E4M3: one byte a value and, per (page, head, slot), one byte E in k_exp / v_exp ([n_pages][n_heads][page_size],
  *   contiguous): value = code * 2^(E - 127).  E is the least for which max |x| of the row <= 448 * 2^(E - 127) (at least
